@@ -1,0 +1,261 @@
+// rope.hip — rotary positions of q and k rows: both pair layouts, part of a head, any frequencies.
+//
+// A head's first rot_dim values are rot_dim / 2 pairs; pair i of a row at position p is turned by the
+// angle a = p * freqs[i] and scaled by m (the magnitude that stretched contexts multiply cos and sin by):
+//   y1 = m (x1 cos a - x2 sin a),  y2 = m (x2 cos a + x1 sin a)
+// half layout: pair i = (x[i], x[i + rot_dim / 2]); interleaved: (x[2 i], x[2 i + 1]). Values past rot_dim
+// are copied. inverse turns by -a with the same m: the transpose, hence the gradient of the call.
+//
+// Angles. A position of 10^6 times a frequency near 1 has no correct bits left after 2^-24 * 10^6 rad in
+// f32, so the product is formed in f64 and reduced there to the nearest quarter turn; what is left
+// (|r| <= 1/8 turn) is rounded to f32 once (2^-28 turns) and goes through sincospif. Two f64 operations a
+// pair and row, shared by all heads of the row: no table, no limit on positions.
+//
+// Bound by HBM: each value is read and written once (2 * rows * heads * D * size bytes). A thread owns one
+// 16-byte chunk of pairs of one row and walks the heads with the same sines and cosines; few rows are
+// spread over the heads instead (a thread a head), where the call is one launch's latency.
+#include <math.h>
+
+#include "common.h"
+
+namespace e2mi {
+
+struct RopeSide {
+    const void *x;
+    void *y;
+    int64_t ldx, ldy;
+};
+struct RopeArgs {
+    RopeSide q, k;
+    int H, KV, M, D, rot;
+    const int32_t *pos;
+    const double *freqs;
+    float mag;
+    int inverse;
+    int hpb;  // heads (of H + KV) per thread
+};
+
+template <class T>
+__device__ inline T from_f32(float v) { return (T)v; }
+
+// sine and cosine of pos * freq, times the magnitude
+__device__ inline void turn(int pos, double freq, float mag, bool inverse, float &c, float &s) {
+    const double t = (double)pos * (freq * 0.15915494309189535);  // turns
+    const double n = __builtin_rint(4.0 * t);
+    const float r = (float)(t - 0.25 * n);
+    float s0, c0;
+    sincospif(2.0f * r, &s0, &c0);
+    const int quarter = (int)(n - 4.0 * __builtin_floor(0.25 * n));
+    const float s1 = quarter & 1 ? c0 : s0, c1 = quarter & 1 ? s0 : c0;
+    s = quarter & 2 ? -s1 : s1;
+    c = (quarter + 1) & 2 ? -c1 : c1;
+    s *= inverse ? -mag : mag;
+    c *= mag;
+}
+
+// V pairs (half layout) or V / 2 pairs (interleaved) of V-element chunks per thread; V = 1 takes one pair
+// in either layout with element loads, for sizes and addresses off 16 bytes.
+template <class T, int V, bool HALF>
+__global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    constexpr bool kPairs = V == 1 || HALF;           // a thread holds whole chunks of both partners
+    constexpr int NP = V == 1 ? 1 : HALF ? V : V / 2;  // pairs per thread
+    const int half = a.rot / 2;
+    const int turned = half / NP;                               // threads that turn pairs, per row
+    const int rest = a.D - a.rot;
+    const int chunks = turned + (rest + V - 1) / V;             // the others copy
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = id / chunks;
+    if (row >= a.M) return;
+    const int ch = (int)(id - row * chunks);
+    const int h0 = blockIdx.y * a.hpb, h1 = min(h0 + a.hpb, a.H + a.KV);
+    auto in = [&](int h) {
+        return h < a.H ? (const T *)a.q.x + row * a.q.ldx + (int64_t)h * a.D : (const T *)a.k.x + row * a.k.ldx + (int64_t)(h - a.H) * a.D;
+    };
+    auto out = [&](int h) {
+        return h < a.H ? (T *)a.q.y + row * a.q.ldy + (int64_t)h * a.D : (T *)a.k.y + row * a.k.ldy + (int64_t)(h - a.H) * a.D;
+    };
+    if (ch >= turned) {
+        const int d = a.rot + (ch - turned) * V;
+        for (int h = h0; h < h1; h++) {
+            const T *x = in(h);
+            T *y = out(h);
+            if (x != y) *(vec *)(y + d) = *(const vec *)(x + d);
+        }
+        return;
+    }
+    float c[NP], s[NP];
+    const int pos = a.pos[row];
+#pragma unroll
+    for (int i = 0; i < NP; i++) turn(pos, a.freqs[ch * NP + i], a.mag, a.inverse, c[i], s[i]);
+    if constexpr (kPairs) {
+        const int d1 = V == 1 && !HALF ? 2 * ch : ch * V, d2 = V == 1 && !HALF ? d1 + 1 : d1 + half;
+        for (int h = h0; h < h1; h++) {
+            const T *x = in(h);
+            T *y = out(h);
+            const vec u = *(const vec *)(x + d1), v = *(const vec *)(x + d2);
+            vec yu, yv;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float f = (float)u[i], g = (float)v[i];
+                yu[i] = from_f32<T>(__builtin_fmaf(f, c[i], -g * s[i]));
+                yv[i] = from_f32<T>(__builtin_fmaf(g, c[i], f * s[i]));
+            }
+            *(vec *)(y + d1) = yu;
+            *(vec *)(y + d2) = yv;
+        }
+    } else {
+        for (int h = h0; h < h1; h++) {
+            const T *x = in(h);
+            T *y = out(h);
+            const vec u = *(const vec *)(x + ch * V);
+            vec yu;
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const float f = (float)u[2 * i], g = (float)u[2 * i + 1];
+                yu[2 * i] = from_f32<T>(__builtin_fmaf(f, c[i], -g * s[i]));
+                yu[2 * i + 1] = from_f32<T>(__builtin_fmaf(g, c[i], f * s[i]));
+            }
+            *(vec *)(y + ch * V) = yu;
+        }
+    }
+}
+
+// Whether rows of `wa` elements at `a` (pitch lda) can meet rows of `wb` at `b` (pitch ldb): not where their
+// extents lie apart, nor where they are apart as columns of rows of one pitch.
+static bool rows_meet(const void *a, int64_t lda, int64_t wa, const void *b, int64_t ldb, int64_t wb, int64_t M, int size) {
+    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+    const uintptr_t ea = pa + ((M - 1) * lda + wa) * size, eb = pb + ((M - 1) * ldb + wb) * size;
+    if (ea <= pb || eb <= pa) return false;
+    if (lda != ldb) return true;
+    const int64_t pitch = lda * size, d = (int64_t)((pb - pa) % (uintptr_t)pitch);
+    const int64_t off = pb >= pa ? d : (pitch - (int64_t)((pa - pb) % (uintptr_t)pitch)) % pitch;
+    return !(off >= wa * size && off + wb * size <= pitch);
+}
+
+template <class T, int V, bool HALF>
+static int launch_rope(hipStream_t st, RopeArgs a) {
+    constexpr int NP = V == 1 ? 1 : HALF ? V : V / 2;
+    const int64_t chunks = a.rot / 2 / NP + (a.D - a.rot + V - 1) / V;
+    const int64_t blocks = (chunks * a.M + 255) / 256;
+    if (blocks > 0x7fffffff) {
+        set_error("rope: too many rows (M=%d D=%d)", a.M, a.D);
+        return -1;
+    }
+    // heads per thread: all where the rows alone give every CU four workgroups, fewer below
+    const int heads = a.H + a.KV;
+    int64_t split = (4L * num_cus() + blocks - 1) / blocks;
+    if (split > heads) split = heads;
+    a.hpb = (int)((heads + split - 1) / split);
+    const int ny = (heads + a.hpb - 1) / a.hpb;
+    hipLaunchKernelGGL((k_rope<T, V, HALF>), dim3((unsigned)blocks, ny), dim3(256), 0, st, a);
+    return check_hip(hipGetLastError(), "rope launch");
+}
+
+template <class T>
+static int rope_typed(hipStream_t st, const RopeArgs &a, bool half) {
+    constexpr int V = 16 / sizeof(T);
+    auto fits = [&](const RopeSide &s) {
+        return !s.x || (aligned16(s.x) && aligned16(s.y) && s.ldx % V == 0 && s.ldy % V == 0);
+    };
+    // 16-byte chunks where every head, both partners and the rest start on one
+    const bool wide = a.D % V == 0 && a.rot % (half ? 2 * V : V) == 0 && fits(a.q) && fits(a.k);
+    if (half) return wide ? launch_rope<T, V, true>(st, a) : launch_rope<T, 1, true>(st, a);
+    return wide ? launch_rope<T, V, false>(st, a) : launch_rope<T, 1, false>(st, a);
+}
+
+}  // namespace e2mi
+
+using namespace e2mi;
+
+extern "C" int e2mi_rope_freqs(double *freqs, int rot_dim, double theta, int scaling, double factor, int trained_len,
+                               double turns_lo, double turns_hi) {
+    if (!freqs || rot_dim <= 0 || rot_dim % 2 || !(theta > 0.0) || !(theta < INFINITY) || scaling < 0 || scaling > 3) {
+        set_error("rope_freqs: needs freqs, an even rot_dim > 0, a finite theta > 0 and a scaling of 0 .. 3 (rot_dim=%d "
+                  "theta=%g scaling=%d)", rot_dim, theta, scaling);
+        return -1;
+    }
+    if (scaling != E2MI_ROPE_PLAIN && (!(factor > 0.0) || !(factor < INFINITY))) {
+        set_error("rope_freqs: needs a finite factor > 0 (%g)", factor);
+        return -1;
+    }
+    if (scaling == E2MI_ROPE_BASE && rot_dim <= 2) {
+        set_error("rope_freqs: the base can be scaled with more than one pair only (rot_dim=%d)", rot_dim);
+        return -1;
+    }
+    if (scaling == E2MI_ROPE_PARTS && (trained_len <= 0 || !(turns_lo >= 0.0) || !(turns_hi > turns_lo) || !(turns_hi < INFINITY))) {
+        set_error("rope_freqs: scaling by parts needs trained_len > 0 and 0 <= turns_lo < turns_hi (%d, %g, %g)", trained_len,
+                  turns_lo, turns_hi);
+        return -1;
+    }
+    const double base = scaling == E2MI_ROPE_BASE ? theta * pow(factor, rot_dim / (rot_dim - 2.0)) : theta;
+    for (int i = 0; i < rot_dim / 2; i++) {
+        double f = pow(base, -2.0 * i / rot_dim);
+        if (scaling == E2MI_ROPE_LINEAR) f /= factor;
+        if (scaling == E2MI_ROPE_PARTS) {
+            const double turns = trained_len * f / 6.283185307179586;
+            double keep = (turns - turns_lo) / (turns_hi - turns_lo);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            f = f * keep + f / factor * (1.0 - keep);
+        }
+        freqs[i] = f;
+    }
+    return 0;
+}
+
+extern "C" int e2mi_rope(e2mi_stream stream, int dtype, int layout, int inverse, const void *q, int64_t ldq, void *q_out,
+                         int64_t ldq_out, int H, const void *k, int64_t ldk, void *k_out, int64_t ldk_out, int KV, int M,
+                         int D, const int32_t *pos, const double *freqs, int rot_dim, float magnitude) {
+    if (dtype < E2MI_F16 || dtype > E2MI_F32 || layout < E2MI_ROPE_HALF || layout > E2MI_ROPE_INTERLEAVED) {
+        set_error("rope: unknown type %d or layout %d", dtype, layout);
+        return -1;
+    }
+    if (M < 0 || D <= 0 || D > 65536 || H < 0 || KV < 0 || H > 65535 || KV > 65535 - H || H + KV == 0 || rot_dim <= 0 ||
+        rot_dim % 2 || rot_dim > D || !(magnitude > -INFINITY) || !(magnitude < INFINITY)) {
+        set_error("rope: needs M >= 0, heads, an even 0 < rot_dim <= D and a finite magnitude (M=%d H=%d KV=%d D=%d rot_dim=%d)",
+                  M, H, KV, D, rot_dim);
+        return -1;
+    }
+    const int size = dtype == E2MI_F32 ? 4 : 2;
+    RopeArgs a = {};
+    a.q = {q, q_out, ldq, ldq_out};
+    a.k = {k, k_out, ldk, ldk_out};
+    a.H = H, a.KV = KV, a.M = M, a.D = D, a.rot = rot_dim;
+    a.pos = pos, a.freqs = freqs, a.mag = magnitude, a.inverse = inverse != 0;
+    if (!H) a.q = {};
+    if (!KV) a.k = {};
+    const RopeSide *side[2] = {&a.q, &a.k};
+    const int heads[2] = {H, KV};
+    for (int i = 0; i < 2; i++) {
+        const int64_t w = (int64_t)heads[i] * D;
+        if (!heads[i]) continue;
+        if (!side[i]->x || !side[i]->y || ((uintptr_t)side[i]->x | (uintptr_t)side[i]->y) % size || side[i]->ldx < w ||
+            side[i]->ldy < w || side[i]->ldx > (1LL << 28) || side[i]->ldy > (1LL << 28)) {
+            set_error("rope: %s needs non-null, aligned rows with a pitch of at least heads * D", i ? "k" : "q");
+            return -1;
+        }
+    }
+    if (!pos || !freqs || (uintptr_t)pos % 4 || (uintptr_t)freqs % 8) {
+        set_error("rope: null or misaligned positions or frequencies");
+        return -1;
+    }
+    if (M == 0) return 0;
+    // in place or apart: an output row may be its own input row, and nothing else that the call reads or writes
+    for (int i = 0; i < 2; i++)
+        for (int j = 0; j < 2; j++) {
+            if (!heads[i] || !heads[j]) continue;
+            const RopeSide &s = *side[i], &t = *side[j];
+            const int64_t ws = (int64_t)heads[i] * D, wt = (int64_t)heads[j] * D;
+            const bool own = i == j && s.y == s.x && s.ldy == s.ldx;
+            if ((!own && rows_meet(s.y, s.ldy, ws, t.x, t.ldx, wt, M, size)) ||
+                (i < j && rows_meet(s.y, s.ldy, ws, t.y, t.ldy, wt, M, size))) {
+                set_error("rope: an output overlaps another operand (in place needs the same rows and pitch)");
+                return -1;
+            }
+        }
+    const hipStream_t st = (hipStream_t)stream;
+    const bool half = layout == E2MI_ROPE_HALF;
+    if (dtype == E2MI_F16) return rope_typed<_Float16>(st, a, half);
+    if (dtype == E2MI_BF16) return rope_typed<__bf16>(st, a, half);
+    return rope_typed<float>(st, a, half);
+}

@@ -13,7 +13,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libe2mi.so")
 
-_P, _I, _F = C.c_void_p, C.c_int, C.c_float
+_P, _I, _F, _L, _D = C.c_void_p, C.c_int, C.c_float, C.c_int64, C.c_double
 
 
 class Q8W(C.Structure):
@@ -95,6 +95,8 @@ SIGNATURES = {
     "e2mi_attention_i8_packed": (_I, [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I]),
     "e2mi_pool_l2_packed": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P]),
     "e2mi_gather_ids": (_I, [_P, _P, _P, _I, _P]),
+    "e2mi_rope_freqs": (_I, [_P, _I, _D, _I, _D, _I, _D, _D]),
+    "e2mi_rope": (_I, [_P, _I, _I, _I, _P, _L, _P, _L, _I, _P, _L, _P, _L, _I, _I, _I, _P, _P, _I, _F]),
     # backend-selection surface (include/e2_dispatch.h)
     "e2_dispatch_set_cpu_backend": (None, [_I]),
     "e2_cpu_backend": (_I, []),
@@ -741,6 +743,84 @@ def gather_ids(ids, rowmap, stream=None):
     out = torch.empty(M, dtype=torch.int32, device=rowmap.device)
     check(load().e2mi_gather_ids(_stream(stream), _p(ids), _p(rowmap), M, _p(out)), "gather_ids")
     return out
+
+
+# ---- long contexts: rotary positions, a shared prefix, selected key blocks
+_DTYPES = {}
+
+
+def _dtype(*tensors):
+    """The library's code of the tensors' one type; they lie on the current device, rows contiguous."""
+    import torch
+    if not _DTYPES:
+        _DTYPES.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+    dev, kind = torch._C._cuda_getDevice(), tensors[0].dtype
+    for t in tensors:
+        if t.dtype != kind or kind not in _DTYPES:
+            raise E2MIError(f"needs tensors of one type (f16, bf16 or f32), got {t.dtype} with {kind}")
+        if t.device.type != "cuda" or t.get_device() != dev:
+            raise E2MIError(f"needs tensors on the current device {dev}, got one on {t.device}")
+        if t.stride(-1) != 1 and t.shape[-1] != 1:
+            raise E2MIError("needs rows of contiguous values")
+    return _DTYPES[kind]
+
+
+def _i32(dev, n, **named):
+    """Checks of device index arrays: int32, contiguous, on the tensors' device, n entries."""
+    import torch
+    for name, t in named.items():
+        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous() or t.numel() < n:
+            raise E2MIError(f"{name} needs at least {n} contiguous int32 values on {dev}")
+
+
+def rope_freqs(rot_dim, theta=10000.0, scaling="plain", factor=1.0, trained_len=0, turns=(1.0, 32.0)):
+    """Angles per position of rot_dim / 2 pairs (e2mi_rope_freqs), float64 on the host; scaling "plain",
+    "linear", "base" or "parts"."""
+    import numpy as np
+    import torch
+    f = np.empty(max(1, rot_dim // 2), np.float64)
+    kind = {"plain": 0, "linear": 1, "base": 2, "parts": 3}[scaling]
+    check(load().e2mi_rope_freqs(ptr(f), rot_dim, theta, kind, factor, trained_len, turns[0], turns[1]), "rope_freqs")
+    return torch.from_numpy(f)
+
+
+def rope(q, k, pos, freqs, H, KV, layout="half", magnitude=1.0, inverse=False, q_out=None, k_out=None, stream=None):
+    """Rotary positions of q [M, H * D] and k [M, KV * D] (e2mi_rope; either may be None): pos int32 [M] and
+    freqs float64 [rot_dim / 2] on the device. Returns (q_out, k_out), new tensors unless given (in
+    place: q_out=q)."""
+    import torch
+    given = [t for t in (q, k, q_out, k_out) if t is not None]
+    if q is None and k is None:
+        raise E2MIError("rope: needs q or k")
+    kind = _dtype(*given)
+    x = q if q is not None else k
+    M, dev = x.shape[0], x.device
+    D = q.shape[1] // H if q is not None else k.shape[1] // KV
+    for t, n in ((q, H), (q_out, H), (k, KV), (k_out, KV)):
+        if t is not None and (t.dim() != 2 or t.shape[0] != M or t.shape[1] != n * D):
+            raise E2MIError(f"rope: needs rows [{M}, {n} * {D}], got {tuple(t.shape)}")
+    _i32(dev, M, pos=pos)
+    if freqs.dtype != torch.float64 or freqs.device != dev or not freqs.is_contiguous():
+        raise E2MIError(f"rope: needs contiguous float64 frequencies on {dev}")
+    if q is not None and q_out is None:
+        q_out = _on(stream, lambda: torch.empty((M, H * D), dtype=q.dtype, device=dev))
+    if k is not None and k_out is None:
+        k_out = _on(stream, lambda: torch.empty((M, KV * D), dtype=k.dtype, device=dev))
+    ld = lambda t: 0 if t is None else t.stride(0) if M > 1 else max(t.stride(0), t.shape[1])  # noqa: E731
+    check(load().e2mi_rope(_stream(stream), kind, {"half": 0, "interleaved": 1}[layout], int(inverse), _p(q), ld(q),
+                           _p(q_out), ld(q_out), 0 if q is None else H, _p(k), ld(k), _p(k_out), ld(k_out),
+                           0 if k is None else KV, M, D, _p(pos), _p(freqs), 2 * freqs.numel(), magnitude), "rope")
+    return q_out, k_out
+
+
+def _on(stream, make):
+    """A new tensor for work on `stream` (None: the current one): allocated there, so that its memory is not
+    handed to other work before that stream is done with it."""
+    if stream is None:
+        return make()
+    import torch
+    with torch.cuda.stream(stream):
+        return make()
 
 
 # ---- model container and encoder engine

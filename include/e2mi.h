@@ -348,6 +348,36 @@ int e2mi_attention(e2mi_stream stream, const uint16_t *q16, const uint16_t *k16,
                    const uint16_t *vt16, const uint8_t *valid, int B, int S, int H, int KV, int D,
                    float scale, int8_t *ctx_q, float *ctx_s, float *ctx32);
 
+/* ---- long contexts: rotary positions, a shared prefix, selected key blocks
+ *
+ * For callers with their own forward over texts longer than the encoder's max_seq; no counterparts in the
+ * reference, whose RoPE is the half layout over whole heads at unscaled frequencies (kernels.c:112-126) and
+ * whose attention reads every key of its own sequence (text.c:534-572). They take 16-bit rows (f16 or
+ * bf16) of a given pitch, so they run on what e2mi_qkv_norm_rope_packed writes (q16, k16, vt16: pitches H*D,
+ * KV*D and M) and on caches of the caller's own. */
+enum { E2MI_F16 = 0, E2MI_BF16 = 1, E2MI_F32 = 2 };
+enum { E2MI_ROPE_HALF = 0, E2MI_ROPE_INTERLEAVED = 1 };
+enum { E2MI_ROPE_PLAIN = 0, E2MI_ROPE_LINEAR = 1, E2MI_ROPE_BASE = 2, E2MI_ROPE_PARTS = 3 };
+
+/* Host helper: the angle per position of each of rot_dim / 2 pairs, f_i = theta^(-2 i / rot_dim), stretched
+ * for contexts `factor` times the trained one: PLAIN as it is; LINEAR f_i / factor; BASE with theta *
+ * factor^(rot_dim / (rot_dim - 2)); PARTS by how often a pair turns over trained_len positions: pairs of
+ * turns_hi turns and more keep f_i, those of turns_lo and fewer take f_i / factor, linear in the turns
+ * between. factor is read by all but PLAIN, trained_len and the turns by PARTS only. */
+int e2mi_rope_freqs(double *freqs, int rot_dim, double theta, int scaling, double factor, int trained_len,
+                    double turns_lo, double turns_hi);
+/* Rotary positions of q rows [M][H][D] and k rows [M][KV][D] (pitches in elements; H or KV may be 0, its
+ * pointers then NULL): the first rot_dim values of every head are pairs (HALF: i and i + rot_dim / 2;
+ * INTERLEAVED: 2 i and 2 i + 1), pair i of row m turned by pos[m] * freqs[i] and scaled by magnitude; the
+ * others are copied. inverse turns the other way: with the same arguments it maps the gradient of the
+ * outputs to the gradient of the inputs, and with 1 / magnitude it takes rows back to unturned ones. dtype
+ * E2MI_F16, _BF16 or _F32; arithmetic in f32, angles in f64 (any position an int32 holds). pos [M] and
+ * freqs [rot_dim / 2] are device memory. Outputs may be their own inputs (same rows, same pitch), else lie
+ * apart from every operand. */
+int e2mi_rope(e2mi_stream stream, int dtype, int layout, int inverse, const void *q, int64_t ldq, void *q_out,
+              int64_t ldq_out, int H, const void *k, int64_t ldk, void *k_out, int64_t ldk_out, int KV, int M,
+              int D, const int32_t *pos, const double *freqs, int rot_dim, float magnitude);
+
 /* ---- the encoder on the device (e2hip.h:34-64) */
 
 /* This repository's model container (include/e2.h names it e2_model there). It is not the
