@@ -1,0 +1,62 @@
+// attn_keys.h — what the attention kernels over a shared prefix and over selected blocks take, and their plan.
+#pragma once
+
+#include "common.h"
+
+namespace e2mi {
+
+constexpr int kKeyBlock = E2MI_KEY_BLOCK;  // keys of a selectable block
+constexpr int kMaxKeyParts = 64;           // shares of a key range, merged by one wave's lanes
+constexpr int kMaxSelect = 2048;           // entries of a selection list
+
+// Keys of a call: rows [rows][ldk] of K (kv heads side by side) and V transposed, [KV * D][ldv].
+struct KeySet {
+    const uint16_t *k, *vt;
+    int64_t ldk, ldv;
+    int rows;
+};
+
+struct KeysArgs {
+    const uint16_t *q;
+    int64_t ldq;
+    int Mq;
+    KeySet own, pre;  // pre.rows: the prefix's keys (0: none)
+    const int32_t *q_start, *q_len, *k_start, *k_len;
+    int B, max_q, max_k, H, KV, G;  // G = H / KV rows of one token in a kv head's tile
+    float c2;                       // scale * log2(e): logits in base-2 units
+    int causal;
+    // selected blocks: lists [B][NQ][KV][n_sel] for blocks of q_block tokens
+    const int32_t *sel;
+    int q_block, NQ, n_sel;
+    // outputs
+    uint16_t *ctx;
+    int64_t ldc;
+    int8_t *cq;
+    float *cs;
+    // shares: part p of token m, head h at part_o[((p * Mq + m) * H + h) * D], its row max and sum at
+    // part_ml[((p * Mq + m) * H + h) * 2]; this launch writes parts part0 .. part0 + parts - 1 of all
+    float *part_o, *part_ml;
+    int part0, parts, all_parts;
+};
+
+// A sequence's row range, cut to the call's limit; false for none, or for one outside the rows given (read
+// as empty: an access never leaves the tensors, whatever the device arrays hold).
+__device__ inline bool row_range(const int32_t *start, const int32_t *len, int b, int most, int rows, int &s, int &n) {
+    s = start[b];
+    n = min(len[b], most);
+    if (n <= 0 || s < 0 || (int64_t)s + n > rows) {
+        s = n = 0;
+        return false;
+    }
+    return true;
+}
+// The same of keys, whose starts are multiples of 8 (V^T is read in 16-byte chunks).
+__device__ inline bool key_range(const int32_t *start, const int32_t *len, int b, int most, int rows, int &s, int &n) {
+    if (!row_range(start, len, b, most, rows, s, n) || (s & 7)) {
+        s = n = 0;
+        return false;
+    }
+    return true;
+}
+
+}  // namespace e2mi

@@ -97,6 +97,16 @@ SIGNATURES = {
     "e2mi_gather_ids": (_I, [_P, _P, _P, _I, _P]),
     "e2mi_rope_freqs": (_I, [_P, _I, _D, _I, _D, _I, _D, _D]),
     "e2mi_rope": (_I, [_P, _I, _I, _I, _P, _L, _P, _L, _I, _P, _L, _P, _L, _I, _I, _I, _P, _P, _I, _F]),
+    "e2mi_attention_prefix_workspace_bytes": (C.c_size_t, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "e2mi_attention_prefix": (_I, [_P, _I, _P, _L, _I, _P, _L, _P, _L, _I, _P, _L, _P, _L, _I, _P, _P, _P, _P, _I, _I, _I,
+                                   _I, _I, _I, _F, _I, _P, _L, _P, _P, _P, C.c_size_t]),
+    "e2mi_block_bounds": (_I, [_P, _I, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "e2mi_block_select_workspace_bytes": (C.c_size_t, [_I, _I, _I, _I, _I]),
+    "e2mi_block_select": (_I, [_P, _I, _P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P,
+                               C.c_size_t]),
+    "e2mi_attention_blocks_workspace_bytes": (C.c_size_t, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "e2mi_attention_blocks": (_I, [_P, _I, _P, _L, _I, _P, _L, _P, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P,
+                                   _I, _F, _I, _P, _L, _P, _P, _P, C.c_size_t]),
     # backend-selection surface (include/e2_dispatch.h)
     "e2_dispatch_set_cpu_backend": (None, [_I]),
     "e2_cpu_backend": (_I, []),
@@ -821,6 +831,148 @@ def _on(stream, make):
     import torch
     with torch.cuda.stream(stream):
         return make()
+
+
+def _keys_of(name, k, vt, KV, D):
+    """(k, its pitch, vt, its pitch, rows) of keys k [rows, KV * D] and vt [KV, D, columns >= rows]."""
+    if k is None or k.shape[0] == 0:
+        return None, 0, None, 0, 0
+    if k.dim() != 2 or k.shape[1] != KV * D or vt.dim() != 3 or vt.shape[0] != KV or vt.shape[1] != D or vt.shape[2] < k.shape[0]:
+        raise E2MIError(f"{name}: needs k [rows, {KV * D}] and vt [{KV}, {D}, >= rows], got {tuple(k.shape)} and {tuple(vt.shape)}")
+    if vt.stride(0) != D * vt.stride(1):
+        raise E2MIError(f"{name}: needs vt's kv heads one after the other (a head pitch of D rows)")
+    return _p(k), k.stride(0) if k.shape[0] > 1 else max(k.stride(0), KV * D), _p(vt), vt.stride(1), k.shape[0]
+
+
+def _contexts(name, q, H, D, ctx, quant, stream):
+    """The outputs: ctx given, made (zeros, so that rows outside every sequence are defined) or left out for the
+    quantized pair."""
+    import torch
+    M, dev = q.shape[0], q.device
+    if quant:
+        if ctx is not None:
+            raise E2MIError(f"{name}: either ctx or the quantized pair")
+        return None, *_on(stream, lambda: (torch.zeros((M, H * D), dtype=torch.int8, device=dev),
+                                           torch.zeros((M, H * D // 128), dtype=torch.float32, device=dev)))
+    if ctx is None:
+        ctx = _on(stream, lambda: torch.zeros((M, H * D), dtype=q.dtype, device=dev))
+    if ctx.shape != (M, H * D):
+        raise E2MIError(f"{name}: needs ctx [{M}, {H * D}], got {tuple(ctx.shape)}")
+    _dtype(q, ctx)
+    return ctx, None, None
+
+
+def _workspace(need, workspace, dev, stream):
+    """The caller's workspace, or a new one of `need` bytes; (tensor, address, bytes)."""
+    import torch
+    if workspace is None:
+        if not need:
+            return None, None, 0
+        workspace = _on(stream, lambda: torch.empty(need, dtype=torch.uint8, device=dev))
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise E2MIError(f"needs a contiguous workspace on {dev}")
+    return workspace, _p(workspace), workspace.numel() * workspace.element_size()
+
+
+def _ld(t, width):
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+def attention_prefix(q, k, vt, pk, pvt, q_start, q_len, max_q, H, KV, k_start=None, k_len=None, max_k=None, scale=1.0,
+                     causal=False, ctx=None, quant=False, workspace=None, stream=None):
+    """Attention of packed sequences over a shared prefix and their own keys (e2mi_attention_prefix): q [Mq, H * D],
+    own keys k [Mk, KV * D] and vt [KV, D, >= Mk] (k None: none), the prefix's pk [P, KV * D] and pvt
+    [KV, D, >= P] (None: none); ranges int32 [B] on the device, key ranges those of q unless given. Returns
+    ctx [Mq, H * D] (new unless given), or with quant the pair (int8 [Mq, H * D], f32 scales per 128)."""
+    lib = load()
+    D = q.shape[1] // H
+    keys = [t for t in (k, vt, pk, pvt) if t is not None]
+    kind = _dtype(q, *keys)
+    if q.dim() != 2 or q.shape[1] != H * D:
+        raise E2MIError(f"attention_prefix: needs q [rows, {H} heads], got {tuple(q.shape)}")
+    k_start, k_len = q_start if k_start is None else k_start, q_len if k_len is None else k_len
+    max_k = max_q if max_k is None else max_k
+    B, Mq = q_start.shape[0], q.shape[0]
+    _i32(q.device, B, q_start=q_start, q_len=q_len, k_start=k_start, k_len=k_len)
+    own, pre = _keys_of("attention_prefix", k, vt, KV, D), _keys_of("attention_prefix", pk, pvt, KV, D)
+    ctx, cq, cs = _contexts("attention_prefix", q, H, D, ctx, quant, stream)
+    ws, wp, wn = _workspace(lib.e2mi_attention_prefix_workspace_bytes(Mq, pre[4], B, max_q, max_k, H, KV, D), workspace, q.device,
+                            stream)
+    check(lib.e2mi_attention_prefix(_stream(stream), kind, _p(q), _ld(q, H * D), Mq, *own, *pre, _p(q_start), _p(q_len),
+                                    _p(k_start), _p(k_len), B, max_q, max_k, H, KV, D, scale, int(causal), _p(ctx),
+                                    0 if ctx is None else _ld(ctx, H * D), _p(cq), _p(cs), wp, wn), "attention_prefix")
+    return ctx if ctx is not None else (cq, cs)
+
+
+def block_bounds(k, k_start, k_len, max_k, KV, bounds=None, stream=None):
+    """Bounds of every block of 64 keys (e2mi_block_bounds): (int8 [B, ceil(max_k / 64), KV, 2 * D], f32 [B, .., KV]),
+    new (zeros) unless given."""
+    import torch
+    kind = _dtype(k)
+    D, B, NB = k.shape[1] // KV, k_start.shape[0], (max_k + 63) // 64
+    _i32(k.device, B, k_start=k_start, k_len=k_len)
+    if bounds is None:
+        bounds = _on(stream, lambda: (torch.zeros((B, NB, KV, 2 * D), dtype=torch.int8, device=k.device),
+                                      torch.zeros((B, NB, KV), dtype=torch.float32, device=k.device)))
+    _check_bounds("block_bounds", bounds, B, NB, KV, D, k.device)
+    check(load().e2mi_block_bounds(_stream(stream), kind, _p(k), _ld(k, KV * D), k.shape[0], _p(k_start), _p(k_len), B, max_k, KV,
+                                   D, _p(bounds[0]), _p(bounds[1])), "block_bounds")
+    return bounds
+
+
+def _check_bounds(name, bounds, B, NB, KV, D, dev):
+    import torch
+    b, s = bounds
+    if (b.shape != (B, NB, KV, 2 * D) or s.shape != (B, NB, KV) or b.dtype != torch.int8 or s.dtype != torch.float32 or
+            b.device != dev or s.device != dev or not b.is_contiguous() or not s.is_contiguous()):
+        raise E2MIError(f"{name}: needs contiguous bounds int8 [{B}, {NB}, {KV}, {2 * D}] and f32 [{B}, {NB}, {KV}] on {dev}")
+
+
+def block_select(q, bounds, q_start, q_len, k_len, max_q, max_k, H, KV, q_block, n_sel, n_first=0, n_local=0, causal=False,
+                 sel=None, workspace=None, stream=None):
+    """The blocks each block of q_block queries reads (e2mi_block_select) from block_bounds' pair: sel int32
+    [B, ceil(max_q / q_block), KV, n_sel], ascending, -1 past the last."""
+    import torch
+    lib = load()
+    kind = _dtype(q)
+    D, B, dev = q.shape[1] // H, q_start.shape[0], q.device
+    _i32(dev, B, q_start=q_start, q_len=q_len, k_len=k_len)
+    _check_bounds("block_select", bounds, B, (max_k + 63) // 64, KV, D, dev)
+    shape = (B, (max_q + max(q_block, 1) - 1) // max(q_block, 1), KV, max(n_sel, 0))
+    if sel is None:
+        sel = _on(stream, lambda: torch.empty(shape, dtype=torch.int32, device=dev))
+    if sel.shape != shape:
+        raise E2MIError(f"block_select: needs sel {shape}, got {tuple(sel.shape)}")
+    _i32(dev, 0, sel=sel)
+    ws, wp, wn = _workspace(lib.e2mi_block_select_workspace_bytes(B, max_q, max_k, KV, q_block), workspace, dev, stream)
+    check(lib.e2mi_block_select(_stream(stream), kind, _p(q), _ld(q, H * D), q.shape[0], _p(bounds[0]), _p(bounds[1]), _p(q_start),
+                                _p(q_len), _p(k_len), B, max_q, max_k, H, KV, D, q_block, n_sel, n_first, n_local, int(causal),
+                                _p(sel), wp, wn), "block_select")
+    return sel
+
+
+def attention_blocks(q, k, vt, sel, q_start, q_len, k_start, k_len, max_q, max_k, H, KV, q_block, scale=1.0, causal=False, ctx=None,
+                     quant=False, workspace=None, stream=None):
+    """Attention over the listed blocks of 64 keys (e2mi_attention_blocks): sel as block_select gives it. Returns as
+    attention_prefix."""
+    lib = load()
+    D, B, Mq, dev = q.shape[1] // H, q_start.shape[0], q.shape[0], q.device
+    kind = _dtype(q, k, vt)
+    if q.dim() != 2 or q.shape[1] != H * D:
+        raise E2MIError(f"attention_blocks: needs q [rows, {H} heads], got {tuple(q.shape)}")
+    if sel.dim() != 4 or sel.shape[:3] != (B, (max_q + max(q_block, 1) - 1) // max(q_block, 1), KV):
+        raise E2MIError(f"attention_blocks: needs sel [B, query blocks, {KV}, n], got {tuple(sel.shape)}")
+    _i32(dev, B, q_start=q_start, q_len=q_len, k_start=k_start, k_len=k_len)
+    _i32(dev, 0, sel=sel)
+    own = _keys_of("attention_blocks", k, vt, KV, D)
+    ctx, cq, cs = _contexts("attention_blocks", q, H, D, ctx, quant, stream)
+    n_sel = sel.shape[3]
+    ws, wp, wn = _workspace(lib.e2mi_attention_blocks_workspace_bytes(Mq, B, max_q, H, KV, D, q_block, n_sel), workspace, dev,
+                            stream)
+    check(lib.e2mi_attention_blocks(_stream(stream), kind, _p(q), _ld(q, H * D), Mq, *own, _p(q_start), _p(q_len), _p(k_start),
+                                    _p(k_len), B, max_q, max_k, H, KV, D, q_block, _p(sel), n_sel, scale, int(causal), _p(ctx),
+                                    0 if ctx is None else _ld(ctx, H * D), _p(cq), _p(cs), wp, wn), "attention_blocks")
+    return ctx if ctx is not None else (cq, cs)
 
 
 # ---- model container and encoder engine

@@ -378,6 +378,69 @@ int e2mi_rope(e2mi_stream stream, int dtype, int layout, int inverse, const void
               int64_t ldq_out, int H, const void *k, int64_t ldk, void *k_out, int64_t ldk_out, int KV, int M,
               int D, const int32_t *pos, const double *freqs, int rot_dim, float magnitude);
 
+/* Packed rows in the entries below: sequence b holds q rows [q_start[b], q_start[b] + q_len[b]) of Mq and keys
+ * [k_start[b], k_start[b] + k_len[b]) of Mk (rows of K, columns of V^T; every k_start a multiple of 8; q and
+ * k ranges may be the same arrays), q_len[b] <= max_q and k_len[b] <= max_k: a longer range is cut, one
+ * outside the rows given or off a multiple of 8 reads as empty. Rows of q are [H][D], of k [KV][D], head h
+ * reads kv head h / (H / KV), vt is [KV][D][ldv] (any pitch of at least its rows); D 64, 128, 256 or 512;
+ * dtype E2MI_F16 or E2MI_BF16 (bits in uint16_t); pitches in elements, those of rows multiples of 8, rows
+ * 16-byte aligned. causal: query i of a sequence reads its own keys j <= i + k_len - q_len (the ends aligned). A row
+ * that sees no key gets a context of 0; rows outside every sequence are not written, and no value outside a
+ * sequence's keys (of any bits) changes a result. Softmax and sums are f32. The context goes to ctx [Mq][H][D]
+ * (dtype, pitch ldc) and / or, quantized per 128 dims for the O projection (D % 128 == 0), to ctx_q
+ * [Mq][H*D] / ctx_s [Mq][H*D/128]; a NULL is left out. Two calls may run at once with a workspace each. */
+
+/* Attention over a prefix that every sequence of the batch reads before its own keys: context of
+ * softmax(scale * q . [prefix | own]) . v, the prefix's P keys (pk rows, pvt columns from 0) all visible, own
+ * keys subject to causal. Positions are in the rows (turned by the caller; e2mi_rope). The prefix's keys are
+ * kept once; sequences of a few rows are also computed against it together, a pass over its keys for all, its
+ * key range shared out over the device where rows are few. P or Mk may be 0. */
+size_t e2mi_attention_prefix_workspace_bytes(int Mq, int P, int B, int max_q, int max_k, int H, int KV, int D);
+int e2mi_attention_prefix(e2mi_stream stream, int dtype, const uint16_t *q, int64_t ldq, int Mq,
+                          const uint16_t *k, int64_t ldk, const uint16_t *vt, int64_t ldv, int Mk,
+                          const uint16_t *pk, int64_t ldpk, const uint16_t *pvt, int64_t ldpv, int P,
+                          const int32_t *q_start, const int32_t *q_len, const int32_t *k_start,
+                          const int32_t *k_len, int B, int max_q, int max_k, int H, int KV, int D, float scale,
+                          int causal, uint16_t *ctx, int64_t ldc, int8_t *ctx_q, float *ctx_s, void *workspace,
+                          size_t workspace_bytes);
+
+/* Attention over selected blocks of E2MI_KEY_BLOCK keys: block n of a sequence is its keys [64 n, 64 n + 64).
+ * Three steps: bounds of the blocks (kept beside the keys, redone for blocks that changed), a selection per
+ * q_block consecutive queries and kv head, the attention over it. */
+enum { E2MI_KEY_BLOCK = 64 };
+/* Bounds of every block: per dim the largest and the smallest key value, quantized together per block and kv
+ * head (amax / 127, ties to even): bounds [B][ceil(max_k / 64)][KV][2][D] (largest, smallest; 16-byte aligned)
+ * and scale [B][ceil(max_k / 64)][KV]. Blocks past a sequence's keys are left as they are. A NaN key value is
+ * passed over. */
+int e2mi_block_bounds(e2mi_stream stream, int dtype, const uint16_t *k, int64_t ldk, int Mk,
+                      const int32_t *k_start, const int32_t *k_len, int B, int max_k, int KV, int D,
+                      int8_t *bounds, float *scale);
+/* The n_sel blocks per query block (sel, as e2mi_attention_blocks reads it) whose bound promises the largest
+ * logits: q rows quantized per (row, head) to q8 and qs, score(n) = max over the query block's rows and the kv
+ * head's query heads of (sum_d max(q8 hi8, q8 lo8)) * qs, times the block's scale, each product rounded to f32;
+ * ties go to the lowest block, lists are in ascending order and end with -1 where there are fewer. causal: a
+ * row scores blocks up to its own place (i + k_len - q_len) only. The first n_first blocks and, for n_local >
+ * 0, those at the query block's own places with n_local - 1 neighbours on each side (causal: before it) are
+ * always taken; together they must fit in n_sel. max_k <= 2^21. The bounds are those of the same max_k. */
+size_t e2mi_block_select_workspace_bytes(int B, int max_q, int max_k, int KV, int q_block);
+int e2mi_block_select(e2mi_stream stream, int dtype, const uint16_t *q, int64_t ldq, int Mq,
+                      const int8_t *bounds, const float *scale, const int32_t *q_start, const int32_t *q_len,
+                      const int32_t *k_len, int B, int max_q, int max_k, int H, int KV, int D, int q_block,
+                      int n_sel, int n_first, int n_local, int causal, int32_t *sel, void *workspace,
+                      size_t workspace_bytes);
+/* Attention of each query over the keys of the blocks listed for its query block (query block i of a
+ * sequence: its tokens [i * q_block, (i + 1) * q_block)): sel [B][ceil(max_q / q_block)][KV][n_sel], n_sel <=
+ * 2048, q_block <= 1024; entries below 0 or past the sequence's last block are passed over, an entry that is
+ * listed twice counts its keys twice. */
+size_t e2mi_attention_blocks_workspace_bytes(int Mq, int B, int max_q, int H, int KV, int D, int q_block,
+                                             int n_sel);
+int e2mi_attention_blocks(e2mi_stream stream, int dtype, const uint16_t *q, int64_t ldq, int Mq,
+                          const uint16_t *k, int64_t ldk, const uint16_t *vt, int64_t ldv, int Mk,
+                          const int32_t *q_start, const int32_t *q_len, const int32_t *k_start,
+                          const int32_t *k_len, int B, int max_q, int max_k, int H, int KV, int D, int q_block,
+                          const int32_t *sel, int n_sel, float scale, int causal, uint16_t *ctx, int64_t ldc,
+                          int8_t *ctx_q, float *ctx_s, void *workspace, size_t workspace_bytes);
+
 /* ---- the encoder on the device (e2hip.h:34-64) */
 
 /* This repository's model container (include/e2.h names it e2_model there). It is not the
