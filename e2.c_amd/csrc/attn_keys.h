@@ -16,7 +16,10 @@ struct KeySet {
     int rows;
 };
 
+enum { kOwnRows = 0, kAllRows = 1, kSelected = 2 };  // a sequence's rows, all rows (the prefix only), listed blocks
+
 struct KeysArgs {
+    int mode;
     const uint16_t *q;
     int64_t ldq;
     int Mq;

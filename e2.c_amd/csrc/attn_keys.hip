@@ -38,7 +38,6 @@ struct Half8<__bf16> {
     static __device__ inline f16v mma(b8 a, b8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
-enum { kOwnRows = 0, kAllRows = 1, kSelected = 2 };  // whose rows against which keys (k_keys_few)
 
 // One tile of the running softmax: 16 logits of one row per lane (its partner lane ^ 32 holds the other 16).
 // The running maximum moves only when a tile exceeds it by more than kTau, so p <= 2^kTau and most tiles need
@@ -72,23 +71,22 @@ __device__ __forceinline__ float softmax_step(const float (&s)[16], float c, flo
 // 8 consecutive values at any 2-byte address (V^T's pitch may be odd): one 16-byte load, unaligned
 template <class T>
 __device__ inline typename Half8<T>::type load8(const uint16_t *p) {
-    struct __attribute__((packed, aligned(2))) Any {
-        typename Half8<T>::type v;
-    };
-    return ((const Any *)p)->v;
+    typename Half8<T>::type v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
 }
 
 __device__ inline int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
 
-// Writes a row's context (a lane holds dims 32 t + 8 g + 4 half + 0..3 of its row, o already divided by the
-// sum): 16-bit rows, and per 128 dims the quantized pair of the O projection.
-template <class T, int D>
-__device__ __forceinline__ void write_row(const KeysArgs &a, const f16v (&o)[D / 32], int64_t m, int h, int half) {
+// Writes DW dims of a row's context from dim0 on (a lane holds dims 32 t + 8 g + 4 half + 0..3 of its row, o already
+// divided by the sum): 16-bit rows, and per 128 dims the quantized pair of the O projection.
+template <class T, int D, int DW = D>
+__device__ __forceinline__ void write_row(const KeysArgs &a, const f16v (&o)[DW / 32], int64_t m, int h, int half, int dim0 = 0) {
     typedef T v4 __attribute__((ext_vector_type(4)));
     if (a.ctx) {
-        T *y = (T *)a.ctx + m * a.ldc + (int64_t)h * D + 4 * half;
+        T *y = (T *)a.ctx + m * a.ldc + (int64_t)h * D + dim0 + 4 * half;
 #pragma unroll
-        for (int t = 0; t < D / 32; t++)
+        for (int t = 0; t < DW / 32; t++)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 const v4 v = {(T)o[t][4 * g], (T)o[t][4 * g + 1], (T)o[t][4 * g + 2], (T)o[t][4 * g + 3]};
@@ -99,7 +97,7 @@ __device__ __forceinline__ void write_row(const KeysArgs &a, const f16v (&o)[D /
         if (a.cq) {
             const int64_t row = m * a.H + h;
 #pragma unroll
-            for (int blk = 0; blk < D / 128; blk++) {
+            for (int blk = 0; blk < DW / 128; blk++) {
                 float am = 0.f;
 #pragma unroll
                 for (int t = 4 * blk; t < 4 * blk + 4; t++)
@@ -111,9 +109,9 @@ __device__ __forceinline__ void write_row(const KeysArgs &a, const f16v (&o)[D /
                 for (int t = 4 * blk; t < 4 * blk + 4; t++)
 #pragma unroll
                     for (int g = 0; g < 4; g++)
-                        *(uint32_t *)(a.cq + row * D + 32 * t + 8 * g + 4 * half) =
+                        *(uint32_t *)(a.cq + row * D + dim0 + 32 * t + 8 * g + 4 * half) =
                             pack4_magic(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3], qs.inv);
-                if (half == 0) a.cs[row * (D / 128) + blk] = qs.sc;
+                if (half == 0) a.cs[row * (D / 128) + dim0 / 128 + blk] = qs.sc;
             }
         }
     }
@@ -137,54 +135,105 @@ __device__ inline int read_list(const int32_t *sel, int n_sel, int blocks, int *
     return *count;
 }
 
-// 32 rows a workgroup; its four waves take every fourth key tile of 32 and are joined through LDS. Fragments
+// A workgroup's rows and keys: which sequence, kv head and tile of rows, and the walk over its key tiles of 32
+// (the prefix's, then its own; or those of a selection list).
+struct Walk {
+    int kvh, b, part;
+    int qs, nq, ks, nk;      // the sequence's rows and own keys
+    int tok0, rows, r0;      // rows of the tile's query block (tokens from tok0), the tile's first
+    int back;                // token i stands at own key i + back
+    int n_pre, t0, t1;       // prefix tiles, this share's tiles
+};
+
+// Fills `w` for a tile of R rows; false where there is no row. list: LDS for a.n_sel entries (kSelected).
+template <int R>
+__device__ inline bool start_walk(const KeysArgs &a, int kvh, int b, int tile, int part, int *list, int *count, Walk &w) {
+    const int G = a.G;
+    w.kvh = kvh, w.b = b, w.part = part;
+    w.qs = 0, w.nq = a.Mq, w.ks = 0, w.nk = 0;
+    if (a.mode != kAllRows) {
+        if (!row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, w.qs, w.nq)) return false;
+        if (a.own.rows) key_range(a.k_start, a.k_len, b, a.max_k, a.own.rows, w.ks, w.nk);
+    }
+    int ntok = w.nq;
+    w.tok0 = 0, w.r0 = tile * R;
+    if (a.mode == kSelected) {
+        const int per = (a.q_block * G + R - 1) / R;
+        w.tok0 = tile / per * a.q_block;
+        ntok = min(a.q_block, w.nq - w.tok0);
+        w.r0 = tile % per * R;
+    }
+    w.rows = ntok * G;
+    if (w.r0 >= w.rows) return false;
+    w.back = w.nk - w.nq;
+    // own keys that any row of the tile sees
+    const int far = a.causal ? min(w.nk, w.tok0 + min(w.r0 + R - 1, w.rows - 1) / G + w.back + 1) : w.nk;
+    int n_own = 0;
+    w.n_pre = 0;
+    if (a.mode == kSelected) {
+        const int32_t *sel = a.sel + (((int64_t)b * a.NQ + w.tok0 / a.q_block) * a.KV + kvh) * a.n_sel;
+        n_own = 2 * read_list(sel, a.n_sel, far > 0 ? (far + kKeyBlock - 1) / kKeyBlock : 0, list, count);
+    } else {
+        w.n_pre = (a.pre.rows + 31) / 32;
+        if (a.mode == kOwnRows && far > 0) n_own = (far + 31) / 32;
+    }
+    const int n = w.n_pre + n_own;
+    w.t0 = (int)((int64_t)n * part / a.parts);
+    w.t1 = (int)((int64_t)n * (part + 1) / a.parts);
+    return true;
+}
+
+// Tile t of a walk: first key of its range and the keys there are (0 for the second half of a short last block).
+struct KeyTile {
+    bool pre;
+    int key0, n;
+};
+__device__ inline KeyTile key_tile(const KeysArgs &a, const Walk &w, const int *list, int t) {
+    KeyTile k;
+    k.pre = t < w.n_pre;
+    if (a.mode == kSelected) k.key0 = list[t >> 1] * kKeyBlock + (t & 1) * 32;
+    else k.key0 = (k.pre ? t : t - w.n_pre) * 32;
+    k.key0 = __builtin_amdgcn_readfirstlane(k.key0);
+    k.n = max(0, min(32, (k.pre ? a.pre.rows : w.nk) - k.key0));
+    return k;
+}
+
+// Leaves a row's share for k_keys_merge: no key: nothing but the maximum says so; a NaN sum (NaN rows) takes the
+// whole row with it.
+template <int D, int DW = D>
+__device__ __forceinline__ void write_share(const KeysArgs &a, const f16v (&o)[DW / 32], float mx, float sum, int part, int64_t m,
+                                            int h, int half, int dim0 = 0) {
+    const int64_t row = ((int64_t)(a.part0 + part) * a.Mq + m) * a.H + h;
+    if (half == 0 && dim0 == 0) *(float2 *)(a.part_ml + row * 2) = make_float2(sum == sum ? mx : INFINITY, sum);
+    if (sum == 0.f) return;
+    float *y = a.part_o + row * D + dim0 + 4 * half;
+#pragma unroll
+    for (int i = 0; i < DW / 32; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *(float4 *)(y + 32 * i + 8 * g) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+}
+
+// Few rows: 32 a workgroup, whose four waves take every fourth key tile and are joined through LDS. Fragments
 // go from global memory to registers: a tile's K and V^T are read by one wave only, so LDS would hold them for
 // nobody else, and the reads in flight are bounded by registers, not by LDS.
-template <class T, int D, int MODE>
+template <class T, int D>
 __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void k_keys_few(KeysArgs a) {
     typedef typename Half8<T>::type V8;
     constexpr int NQ = D / 16, NO = D / 32;
-    extern __shared__ __align__(16) float few_smem[];  // two waves' o (join); the list (kSelected)
+    extern __shared__ __align__(16) float few_smem[];  // the list (kSelected), then two waves' o (join)
     __shared__ float s_m[4][32], s_l[4][32];
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5;
-    const int kvh = blockIdx.y, b = blockIdx.z, G = a.G;
-    const int part = (int)(blockIdx.x % (unsigned)a.parts), tile = (int)(blockIdx.x / (unsigned)a.parts);
-
-    int qs = 0, nq = a.Mq, ks = 0, nk = 0;
-    if constexpr (MODE != kAllRows) {
-        if (!row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, qs, nq)) return;
-        if (a.own.rows) key_range(a.k_start, a.k_len, b, a.max_k, a.own.rows, ks, nk);
-    }
-    // this tile's rows
-    int tok0 = 0, ntok = nq, r0 = tile * 32;
-    if constexpr (MODE == kSelected) {
-        const int per = (a.q_block * G + 31) / 32;
-        tok0 = tile / per * a.q_block;
-        ntok = min(a.q_block, nq - tok0);
-        r0 = tile % per * 32;
-    }
-    const int rows = ntok * G;
-    if (r0 >= rows) return;
-    const int r = r0 + (lane & 31), rc = min(r, rows - 1);
-    const int tok = tok0 + rc / G, h = kvh * G + rc % G;
-    const int64_t m = (int64_t)qs + tok;
-    const int back = nk - nq;  // token i stands at own key i + back
-    const int last = a.causal ? tok + back : nk - 1;
-    const int far = a.causal ? min(nk, tok0 + (min(r0 + 31, rows - 1)) / G + back + 1) : nk;  // own keys any row here sees
-
-    // its key tiles
-    int n_pre = 0, n_own = 0;
     int *list = (int *)few_smem;
-    if constexpr (MODE == kSelected) {
-        const int32_t *sel = a.sel + (((int64_t)b * a.NQ + tok0 / a.q_block) * a.KV + kvh) * a.n_sel;
-        n_own = 2 * read_list(sel, a.n_sel, far > 0 ? (far + kKeyBlock - 1) / kKeyBlock : 0, list, &s_count);
-    } else {
-        n_pre = (a.pre.rows + 31) / 32;
-        if (MODE == kOwnRows && far > 0) n_own = (far + 31) / 32;
-    }
-    const int n = n_pre + n_own;
-    const int t0 = (int)((int64_t)n * part / a.parts), t1 = (int)((int64_t)n * (part + 1) / a.parts);
+    Walk k;
+    if (!start_walk<32>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
+                        &s_count, k))
+        return;
+    const int r = k.r0 + (lane & 31), rc = min(r, k.rows - 1);
+    const int tok = k.tok0 + rc / a.G, h = k.kvh * a.G + rc % a.G;
+    const int64_t m = (int64_t)k.qs + tok;
+    const int last = a.causal ? min(tok + k.back, k.nk - 1) : k.nk - 1;  // own keys this row sees
 
     V8 qf[NQ];
     {
@@ -197,28 +246,23 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void k_keys_few(KeysArgs a) 
     for (int t = 0; t < NO; t++) o[t] = (f16v){};
     float mrun = -INFINITY, lrun = 0.f;
 
-    for (int t = t0 + w; t < t1; t += 4) {
-        const bool pre = t < n_pre;
-        const KeySet &src = pre ? a.pre : a.own;
-        int key0;
-        if constexpr (MODE == kSelected) key0 = list[t >> 1] * kKeyBlock + (t & 1) * 32;
-        else key0 = (pre ? t : t - n_pre) * 32;
-        const int lim = pre ? src.rows : nk;  // keys of this range
-        if (MODE == kSelected && key0 >= lim) continue;
-        const int64_t base = pre ? 0 : ks;
-        const uint16_t *kp = src.k + (base + min(key0 + swap23(lane & 31), lim - 1)) * src.ldk + (int64_t)kvh * D + 8 * half;
+    for (int t = k.t0 + w; t < k.t1; t += 4) {
+        const KeyTile kt = key_tile(a, k, list, t);
+        if (kt.n <= 0) continue;
+        const KeySet &src = kt.pre ? a.pre : a.own;
+        const int64_t row = (kt.pre ? 0 : k.ks) + kt.key0;
+        const uint16_t *kp = src.k + (row + min(swap23(lane & 31), kt.n - 1)) * src.ldk + (int64_t)k.kvh * D + 8 * half;
         f16v st = (f16v){};
 #pragma unroll
         for (int s = 0; s < NQ; s++) st = Half8<T>::mma(*(const V8 *)(kp + 16 * s), qf[s], st);
         float tv[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) tv[i] = st[i];
-        const bool short_tile = key0 + 32 > lim;
-        if (short_tile || (!pre && a.causal)) {
-            const int top = pre ? lim - 1 : min(last, lim - 1);
+        if (kt.n < 32 || (!kt.pre && a.causal)) {
+            const int top = kt.pre ? kt.n - 1 : min(last - kt.key0, kt.n - 1);
 #pragma unroll
             for (int i = 0; i < 16; i++)
-                if (key0 + 16 * (i >> 3) + 8 * half + (i & 7) > top) tv[i] = -INFINITY;
+                if (16 * (i >> 3) + 8 * half + (i & 7) > top) tv[i] = -INFINITY;
         }
         V8 pb[2];
         const float alpha = softmax_step<T>(tv, a.c2, mrun, lrun, pb);
@@ -226,15 +270,15 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void k_keys_few(KeysArgs a) 
 #pragma unroll
             for (int i = 0; i < NO; i++) o[i] *= alpha;
         }
-        const uint16_t *vp = src.vt + ((int64_t)kvh * D + (lane & 31)) * src.ldv + base + key0 + 8 * half;
-        if (!short_tile) {
+        const uint16_t *vp = src.vt + ((int64_t)k.kvh * D + (lane & 31)) * src.ldv + row + 8 * half;
+        if (kt.n == 32) {
 #pragma unroll
             for (int i = 0; i < 2 * NO; i++)
                 o[i >> 1] = Half8<T>::mma(load8<T>(vp + (int64_t)(i >> 1) * 32 * src.ldv + 16 * (i & 1)), pb[i & 1], o[i >> 1]);
         } else {
             // values past the range are not read (they may lie past the tensor) and count as 0: a zero
             // probability times an infinity would be a NaN
-            const int left = lim - key0 - 8 * half;
+            const int left = kt.n - 8 * half;
             for (int i = 0; i < 2 * NO; i++) {
                 const int have = left - 16 * (i & 1);
                 const uint16_t *x = vp + (int64_t)(i >> 1) * 32 * src.ldv + 16 * (i & 1);
@@ -282,24 +326,258 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void k_keys_few(KeysArgs a) 
         }
         if (step > 1) __syncthreads();
     }
-    if (w || r >= rows) return;
+    if (w || r >= k.rows) return;
     if (a.part_o) {
-        const int64_t row = ((int64_t)(a.part0 + part) * a.Mq + m) * a.H + h;
-        // no key: nothing but the maximum says so; a NaN sum (NaN rows) takes the whole row with it
-        if (half == 0) *(float2 *)(a.part_ml + row * 2) = make_float2(lsum == lsum ? mall : INFINITY, lsum);
-        if (lsum == 0.f) return;
-        float *y = a.part_o + row * D + 4 * half;
-#pragma unroll
-        for (int i = 0; i < NO; i++)
-#pragma unroll
-            for (int g = 0; g < 4; g++)
-                *(float4 *)(y + 32 * i + 8 * g) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+        write_share<D>(a, o, mall, lsum, k.part, m, h, half);
         return;
     }
     const float inv = lsum == 0.f ? 0.f : __fdiv_rn(1.f, lsum);
 #pragma unroll
     for (int i = 0; i < NO; i++) o[i] *= inv;
     write_row<T, D>(a, o, m, h, half);
+}
+
+// Many rows: 32 a row group, NW groups that share the key tiles in LDS, fetched one tile ahead by direct-to-LDS
+// loads. Bound by LDS reads as much as by the MFMA unit: a group's 32 rows read all of a tile (128 D bytes, D cycles
+// of the CU's LDS) for 4 D cycles of a SIMD's MFMA, four SIMDs at a time.
+//
+// DS waves a group: at head_dim 512 a wave could not hold 32 rows' Q (128 registers) and context (256), so two
+// waves take half of the dims each, in both products, and add their halves of the logits through LDS.
+//
+// LDS: K tiles of 32 keys x 2 D bytes, V^T tiles of D rows x 64 bytes. K row i holds key swap23(i); its 16-byte
+// chunk x sits at position x ^ (i & 7); chunk c of V^T row d at position c ^ ((d >> 2) & 3): the eight lanes of a
+// read group hit eight bank groups. Two buffers of both; at DS = 2 K has one, which the barrier of the logits'
+// exchange frees, and the exchange takes its place.
+template <int D>
+struct WideTile {
+    static constexpr int DS = D == 512 ? 2 : 1;     // waves that share a row group's dims
+    static constexpr int kTile = 64 * D;            // bytes of a K or V^T tile
+    static constexpr int KB = DS == 1 ? 2 : 1;      // K buffers
+    static constexpr int kV = KB * kTile;           // V^T's two
+    static constexpr int kX = kV + 2 * kTile;       // the exchange: 4 KB a wave
+    static constexpr int bytes(int nw) { return kX + (DS > 1 ? nw * DS * 4096 : 0); }
+};
+__device__ inline void dma16_nc(v4u r, uint32_t lds, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r));
+}
+// K and V^T fragments are read this many MFMAs ahead of their use
+constexpr int kAhead = 3;
+
+template <class T, int D, int NW>
+__global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(KeysArgs a, int tiles) {
+    typedef typename Half8<T>::type V8;
+    using L = WideTile<D>;
+    constexpr int DS = L::DS, WV = NW * DS, DW = D / DS;  // waves, dims of a wave
+    constexpr int NQ = DW / 16, NO = DW / 32;
+    constexpr int RPI = 512 / D, LPR = D / 8;             // K rows a load fetches, lanes per K row
+    constexpr int NL = D / 16, NLW = (NL + WV - 1) / WV;  // loads of a K (or V^T) tile, per wave
+    extern __shared__ __align__(16) unsigned char wide_smem[];
+    __shared__ int s_count;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wu = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int group = wu / DS, dim0 = wu % DS * DW;
+    int *list = (int *)(wide_smem + L::bytes(NW));
+    // consecutive tiles of a sequence read the same keys: they go to one XCD and its L2
+    int id = xcd_swizzle(blockIdx.x, gridDim.x);
+    const int part = id % a.parts;
+    id /= a.parts;
+    const int tile = id % tiles;
+    id /= tiles;
+    Walk k;
+    if (!start_walk<32 * NW>(a, id % a.KV, id / a.KV, tile, part, list, &s_count, k)) return;
+    const int r1 = k.r0 + 32 * group;     // the group's first row
+    const bool active = r1 < k.rows;      // a wave without rows loads its share of the tiles only
+    auto row_of = [&](int l, int &tok, int &h) {
+        const int r = min(r1 + (l & 31), k.rows - 1);
+        tok = k.tok0 + r / a.G;
+        h = k.kvh * a.G + r % a.G;
+    };
+    int last;  // own keys this lane's row sees
+    V8 qf[NQ];
+    {
+        int tok, h;
+        row_of(lane, tok, h);
+        last = a.causal ? min(tok + k.back, k.nk - 1) : k.nk - 1;
+        const uint16_t *qp = a.q + ((int64_t)k.qs + tok) * a.ldq + (int64_t)h * D + dim0 + 8 * half;
+#pragma unroll
+        for (int s = 0; s < NQ; s++) qf[s] = *(const V8 *)(qp + 16 * s);
+    }
+    const int sure = __builtin_amdgcn_readfirstlane(last);  // own keys that all rows of the wave see (its first row's)
+    f16v o[NO];
+#pragma unroll
+    for (int t = 0; t < NO; t++) o[t] = (f16v){};
+    float mrun = -INFINITY, lrun = 0.f;
+
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_void *)wide_smem);
+    const int lr = lane / LPR, lc = lane % LPR;
+    const int vchunk = (lane & 3) ^ ((lane >> 4) & 3);
+    // A tile's loads: load j of a wave takes K rows RPI x .. + RPI - 1 or V^T rows 16 x .. + 15, x = NLW wave + j.
+    // Descriptors start at the load's first row, so 32 bits hold every offset at any length of the cache.
+    struct Fetch {
+        const uint16_t *k, *v;
+        uint32_t ldk, ldv, bytes;  // pitches in bytes; K's range
+        uint32_t ko, vo;           // lane offsets
+    };
+    auto fetch_of = [&](const KeyTile &kt) {
+        const KeySet &src = kt.pre ? a.pre : a.own;
+        const int64_t row = (kt.pre ? 0 : k.ks) + kt.key0;
+        Fetch f;
+        f.k = src.k + row * src.ldk + (int64_t)k.kvh * D;
+        f.v = src.vt + ((int64_t)k.kvh * D + 16 * NLW * wu) * src.ldv + row;
+        f.ldk = (uint32_t)src.ldk * 2, f.ldv = (uint32_t)src.ldv * 2;
+        f.bytes = kt.n ? (uint32_t)(kt.n - 1) * f.ldk + 2 * D : 0;
+        f.ko = (uint32_t)swap23(lr) * f.ldk;
+        f.vo = 8 * vchunk < kt.n ? (uint32_t)(lane >> 2) * f.ldv + (uint32_t)vchunk * 16 : 0x80000000u;
+        return f;
+    };
+    auto load_k = [&](const Fetch &f, int buf, int j) {
+        const int x = NLW * wu + j, i = RPI * x;
+        if (NL % WV && x >= NL) return;
+        // a row past the range reads as zero: the lane offset lies past the descriptor's end
+        const uint32_t key = (uint32_t)swap23(i) * f.ldk;
+        const v4u rs = rsrc_words((const char *)f.k + key, key < f.bytes ? f.bytes - key : 0);
+        dma16_nc(rs, lds0 + (uint32_t)(buf * L::kTile + i * (2 * D)), f.ko + (uint32_t)((lc ^ ((i + lr) & 7)) << 4));
+    };
+    auto load_v = [&](const Fetch &f, int buf, int j) {
+        if (NL % WV && NLW * wu + j >= NL) return;
+        const v4u rs = rsrc_words((const char *)f.v + (uint64_t)(16 * j) * f.ldv, 0x7fffffffu);
+        dma16_nc(rs, lds0 + (uint32_t)(L::kV + buf * L::kTile + (NLW * wu + j) * 1024), f.vo);
+    };
+
+    const int kkey = lane & 31;
+    // fragment reads: K chunk 2 s + half of row kkey (s = 4 t + u: 128 t + ((2 u + half) ^ (kkey & 7)) * 16), V^T chunk
+    // 2 j + half of row kkey of each 32
+    const uint32_t krd = (uint32_t)(kkey * 2 * D + 2 * dim0 + ((half ^ (kkey & 7)) << 4));
+    const uint32_t vrd = (uint32_t)(L::kV + (dim0 + kkey) * 64 + ((half ^ ((kkey >> 2) & 3)) << 4));
+
+    KeyTile now = {}, next = {};
+    Fetch f = {};
+    if (k.t0 < k.t1) {
+        now = key_tile(a, k, list, k.t0);
+        f = fetch_of(now);
+#pragma unroll
+        for (int j = 0; j < NLW; j++) load_k(f, 0, j), load_v(f, 0, j);
+    }
+    // the Q loads are waited for here, by a wait that the compiler's count sees: inside the loop it would cover
+    // the tile loads in flight
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    for (int t = k.t0; t < k.t1; t++, now = next) {
+        const int buf = (t - k.t0) & 1, kbuf = DS == 1 ? buf : 0;
+        // this wave's loads of tile t have landed; the barrier makes every wave's visible and ends every wave's
+        // reads of the buffer that the next loads refill
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const bool more = t + 1 < k.t1;
+        if (more) {
+            next = key_tile(a, k, list, t + 1);
+            f = fetch_of(next);
+        }
+        unsigned char *sk = wide_smem + kbuf * L::kTile, *sv = wide_smem + buf * L::kTile;
+        if (now.n & 7) {  // values past the range in its last chunk (of any bits) become 0
+            for (int d = tid; d < D; d += 64 * WV) {
+                uint32_t *x = (uint32_t *)(sv + L::kV + d * 64 + (((now.n >> 3) ^ ((d >> 2) & 3)) << 4));
+                const int have = now.n & 7;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] &= have >= 2 * e + 2 ? 0xffffffffu : have == 2 * e + 1 ? 0xffffu : 0u;
+            }
+            __syncthreads();
+        }
+        const bool work = active && now.n > 0;
+        f16v st = (f16v){};
+        if (work) {
+            V8 kr[kAhead];
+            auto kfrag = [&](int s) { return *(const V8 *)(sk + (krd ^ (uint32_t)((s & 3) << 5)) + (s >> 2) * 128); };
+#pragma unroll
+            for (int s = 0; s < kAhead; s++) kr[s] = kfrag(s);
+#pragma unroll
+            for (int s = 0; s < NQ; s++) {
+                st = Half8<T>::mma(kr[s % kAhead], qf[s], st);
+                if (s + kAhead < NQ) kr[s % kAhead] = kfrag(s + kAhead);
+                if ((s & 1) && more) {
+                    if ((s >> 1) < NLW) load_v(f, buf ^ 1, s >> 1);
+                    else if (DS == 1 && (s >> 1) < 2 * NLW) load_k(f, buf ^ 1, (s >> 1) - NLW);
+                }
+            }
+        }
+        if (more) {  // what the MFMAs above had no room for
+#pragma unroll
+            for (int j = 0; j < NLW; j++) {
+                if (!work || j >= NQ / 2) load_v(f, buf ^ 1, j);
+                if (DS == 1 && (!work || NLW + j >= NQ / 2)) load_k(f, buf ^ 1, j);
+            }
+        }
+        if constexpr (DS == 2) {
+            float4 *x = (float4 *)(wide_smem + L::kX) + wu * 256 + lane;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[64 * i] = make_float4(st[4 * i], st[4 * i + 1], st[4 * i + 2], st[4 * i + 3]);
+            lds_barrier();  // the K tile is read: its buffer takes the next one
+            if (more)
+#pragma unroll
+                for (int j = 0; j < NLW; j++) load_k(f, 0, j);
+            const float4 *y = (const float4 *)(wide_smem + L::kX) + (wu ^ 1) * 256 + lane;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 v = y[64 * i];
+                st[4 * i] += v.x, st[4 * i + 1] += v.y, st[4 * i + 2] += v.z, st[4 * i + 3] += v.w;
+            }
+        }
+        if (!work) continue;
+        float tv[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) tv[i] = st[i];
+        if (now.n < 32 || (!now.pre && a.causal && now.key0 + 31 > sure)) {
+            const int top = now.pre ? now.n - 1 : min(last - now.key0, now.n - 1);
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (16 * (i >> 3) + 8 * half + (i & 7) > top) tv[i] = -INFINITY;
+        }
+        V8 pb[2];
+        const float alpha = softmax_step<T>(tv, a.c2, mrun, lrun, pb);
+        auto vfrag = [&](int i) { return *(const V8 *)(sv + (vrd ^ (uint32_t)((i & 1) << 5)) + (i >> 1) * 32 * 64); };
+        V8 vr[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) vr[i] = vfrag(i);
+        if (__any(alpha != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < NO; i++) o[i] *= alpha;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * NO; i++) {
+            o[i >> 1] = Half8<T>::mma(vr[i % kAhead], pb[i & 1], o[i >> 1]);
+            if (i + kAhead < 2 * NO) vr[i % kAhead] = vfrag(i + kAhead);
+        }
+    }
+    const float lsum = lrun + xor_lane<32>(lrun);
+    int l = lane;
+    asm volatile("" : "+v"(l));  // the row again, not kept in registers through the loop
+    if (r1 + (l & 31) >= k.rows) return;
+    int tok, h;
+    row_of(l, tok, h);
+    const int64_t m = (int64_t)k.qs + tok;
+    if (a.part_o) {
+        write_share<D, DW>(a, o, mrun, lsum, k.part, m, h, l >> 5, dim0);
+        return;
+    }
+    const float inv = lsum == 0.f ? 0.f : __fdiv_rn(1.f, lsum);
+#pragma unroll
+    for (int i = 0; i < NO; i++) o[i] *= inv;
+    write_row<T, D, DW>(a, o, m, h, l >> 5, dim0);
+}
+
+// V^T rows of any pitch and address, copied to a pitch that 16-byte loads take (k_keys_wide).
+__global__ __launch_bounds__(256) void k_pad_rows(uint16_t *y, int64_t ldy, const uint16_t *x, int64_t ldx, int n) {
+    const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
+    if (c >= n) return;
+    const uint16_t *from = x + row * ldx + c;
+    uint16_t *to = y + row * ldy + c;
+    if (c + 8 <= n) {
+        uint4 v;
+        __builtin_memcpy(&v, from, 16);
+        *(uint4 *)to = v;
+    } else {
+        for (int e = 0; c + e < n; e++) to[e] = from[e];
+    }
 }
 
 // Joins the shares of a row: a wave a row, lane p holding share p's maximum and sum, then D / 64 dims a lane.
@@ -358,87 +636,130 @@ __global__ __launch_bounds__(256) void k_keys_merge(KeysArgs a) {
 
 // ---- host: plan, checks, launches
 
+// How a set of rows runs: nw = 0: k_keys_few, else k_keys_wide with nw waves.
+struct RowsPlan {
+    int nw = 0, parts = 1;
+    int64_t tiles = 0;  // per sequence and kv head
+};
 struct KeysPlan {
-    bool apart = false;           // the prefix by rows of all sequences, their own keys by sequence
-    int pre_parts = 0, parts = 1;  // shares of the prefix (apart) and of the other launch
-    int all() const { return pre_parts + parts; }
-    bool merged() const { return all() > 1; }
+    bool apart = false;  // the prefix by rows of all sequences, their own keys by sequence
+    RowsPlan pre, rows;  // pre: the prefix's launch (apart)
+    size_t pad_pre = 0, pad_own = 0;  // bytes of V^T copies (k_keys_wide over odd pitches)
+    int all() const { return (apart ? pre.parts : 0) + rows.parts; }
 };
 
-// Shares for a launch of `groups` workgroups whose longest walk is `tiles` key tiles of 32: enough to give every
-// CU two workgroups, at least 8 tiles (two a wave) each.
-static int key_shares(int64_t groups, int64_t tiles, int most) {
+// Shares for `groups` workgroups whose longest walk is `tiles` key tiles of 32: enough to give every CU two
+// workgroups, at least `least` tiles each.
+static int key_shares(int64_t groups, int64_t tiles, int least, int most) {
+    if (groups < 1) return 1;
     const int64_t want = (2L * num_cus() + groups - 1) / groups;
-    int64_t n = want < tiles / 8 ? want : tiles / 8;
+    int64_t n = want < tiles / least ? want : tiles / least;
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
 }
 
-static KeysPlan plan_prefix(int Mq, int P, int B, int max_q, int max_k, int H, int KV) {
-    KeysPlan p;
-    const int G = H / KV;
-    const int64_t own_tiles = ((int64_t)max_k + 31) / 32, pre_tiles = ((int64_t)P + 31) / 32;
-    const int64_t seq_groups = (((int64_t)max_q * G + 31) / 32) * KV * B;
-    // sequences of less than a tile share the prefix's tiles
-    p.apart = B > 1 && P > 0 && (int64_t)max_q * G < 32;
-    if (p.apart) {
-        p.pre_parts = key_shares(((int64_t)Mq * G + 31) / 32 * KV, pre_tiles, kMaxKeyParts / 2);
-        p.parts = key_shares(seq_groups, own_tiles, kMaxKeyParts / 2);
-    } else {
-        p.parts = key_shares(seq_groups, own_tiles + pre_tiles, kMaxKeyParts);
-    }
+// groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles
+static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int most, bool wide) {
+    RowsPlan p;
+    p.nw = !wide || rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
+    const int R = p.nw ? 32 * p.nw : 32;
+    p.tiles = (rows + R - 1) / R;
+    p.parts = key_shares(p.tiles * count, tiles, 8, most);
     return p;
 }
 
-static KeysPlan plan_blocks(int B, int max_q, int H, int KV, int q_block, int n_sel) {
+static bool odd_pitch(int64_t ld, int rows) { return rows > 0 && ld % 8; }
+// k_keys_wide's loads are 16 bytes and keep 32-bit offsets within a tile of keys and 16 rows of V^T
+static bool wide_takes(const KeySet &s) {
+    return !s.rows || (s.ldk < (1 << 24) && s.ldv < (1 << 25));
+}
+static size_t pad_bytes(int rows, int KV, int D) { return ((size_t)rows + 7) / 8 * 16 * KV * D; }
+
+static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B, int max_q, int max_k, int H, int KV, int D) {
     KeysPlan p;
-    const int G = H / KV;
-    const int64_t groups = (((int64_t)q_block * G + 31) / 32) * (((int64_t)max_q + q_block - 1) / q_block) * KV * B;
-    p.parts = key_shares(groups, 2 * (int64_t)n_sel, kMaxKeyParts);
+    const int G = H / KV, P = pre.rows;
+    const bool wide = wide_takes(own) && wide_takes(pre);
+    const int64_t own_tiles = own.rows ? ((int64_t)max_k + 31) / 32 : 0, pre_tiles = ((int64_t)P + 31) / 32;
+    const int64_t rows = (int64_t)max_q * G;
+    // sequences of less than a tile share the prefix's tiles
+    p.apart = B > 1 && P > 0 && rows < 32;
+    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, kMaxKeyParts / 2, wide);
+    p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), p.apart ? kMaxKeyParts / 2 : kMaxKeyParts, wide);
+    if (odd_pitch(pre.ldv, P) && (p.apart ? p.pre.nw : p.rows.nw)) p.pad_pre = pad_bytes(P, KV, D);
+    if (odd_pitch(own.ldv, own.rows) && p.rows.nw) p.pad_own = pad_bytes(own.rows, KV, D);
+    return p;
+}
+
+static KeysPlan plan_blocks(const KeySet &own, int B, int max_q, int H, int KV, int D, int q_block, int n_sel) {
+    KeysPlan p;
+    const int64_t NQ = ((int64_t)max_q + q_block - 1) / q_block;
+    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, kMaxKeyParts, wide_takes(own));
+    p.rows.tiles *= NQ;
+    if (odd_pitch(own.ldv, own.rows) && p.rows.nw) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
 }
 
 static size_t part_bytes(const KeysPlan &p, int Mq, int H, int D) {
-    return p.merged() ? (size_t)p.all() * Mq * H * (D + 2) * 4 : 0;
+    return p.all() > 1 ? ((size_t)p.all() * Mq * H * (D + 2) * 4 + 15) / 16 * 16 : 0;
 }
+static size_t workspace_of(const KeysPlan &p, int Mq, int H, int D) { return part_bytes(p, Mq, H, D) + p.pad_pre + p.pad_own; }
 
-template <class T, int D, int MODE>
-static int launch_few(hipStream_t st, const KeysArgs &a, int64_t tiles, int B) {
-    constexpr size_t lds = (size_t)D * 128 * 2 > kMaxSelect * 4 ? (size_t)D * 128 * 2 : kMaxSelect * 4;
-    if (tiles * a.parts > 0x7fffffff) {
-        set_error("attention over keys: too many rows for a launch");
+template <class T, int D, int NW>
+static int launch_wide(hipStream_t st, const KeysArgs &a, int64_t tiles, int64_t grid) {
+    const size_t lds = WideTile<D>::bytes(NW) + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
+    if (check_hip(hipFuncSetAttribute((const void *)k_keys_wide<T, D, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
+                  "lds attribute"))
         return -1;
-    }
-    if (lds > 65536 && check_hip(hipFuncSetAttribute((const void *)k_keys_few<T, D, MODE>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "lds attribute"))
-        return -1;
-    hipLaunchKernelGGL((k_keys_few<T, D, MODE>), dim3((unsigned)(tiles * a.parts), a.KV, B), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((k_keys_wide<T, D, NW>), dim3((unsigned)grid), dim3(64 * NW * WideTile<D>::DS), lds, st, a, (int)tiles);
     return check_hip(hipGetLastError(), "attention launch");
 }
 
 template <class T, int D>
+static int launch_rows(hipStream_t st, KeysArgs a, const RowsPlan &p, int B) {
+    a.parts = p.parts;
+    const int64_t grid = p.tiles * p.parts;
+    if (grid * a.KV * (p.nw ? B : 1) > 0x7fffffff) {
+        set_error("attention over keys: too many rows for a launch");
+        return -1;
+    }
+    if (p.nw == 2) return launch_wide<T, D, 2>(st, a, p.tiles, grid * a.KV * B);
+    if (p.nw == 3) return launch_wide<T, D, 3>(st, a, p.tiles, grid * a.KV * B);
+    if (p.nw == 4) return launch_wide<T, D, 4>(st, a, p.tiles, grid * a.KV * B);
+    const size_t list = a.mode == kSelected ? 4 * (size_t)a.n_sel : 0, join = (size_t)D * 256, lds = list > join ? list : join;
+    if (lds > 65536 && check_hip(hipFuncSetAttribute((const void *)k_keys_few<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                     (int)lds), "lds attribute"))
+        return -1;
+    hipLaunchKernelGGL((k_keys_few<T, D>), dim3((unsigned)grid, a.KV, B), dim3(256), lds, st, a);
+    return check_hip(hipGetLastError(), "attention launch");
+}
+
+// a copy of a set's V^T in rows of 16-byte multiples at `to`
+static int pad_values(hipStream_t st, KeySet &s, int KV, int D, uint16_t *to) {
+    const int64_t ld = ((int64_t)s.rows + 7) / 8 * 8;
+    hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)((ld + 2047) / 2048), D, KV), dim3(256), 0, st, to, ld, s.vt, s.ldv, s.rows);
+    s.vt = to, s.ldv = ld;
+    return check_hip(hipGetLastError(), "V^T copy launch");
+}
+
+template <class T, int D>
 static int run_keys(hipStream_t st, KeysArgs a, const KeysPlan &p, void *workspace) {
-    const int G = a.G;
-    if (p.merged()) {
-        a.part_o = (float *)workspace;
-        a.part_ml = a.part_o + (size_t)p.all() * a.Mq * a.H * D;
-    }
+    char *ws = (char *)workspace + part_bytes(p, a.Mq, a.H, D);
+    if (p.pad_pre && pad_values(st, a.pre, a.KV, D, (uint16_t *)ws)) return -1;
+    if (p.pad_own && pad_values(st, a.own, a.KV, D, (uint16_t *)(ws + p.pad_pre))) return -1;
     a.all_parts = p.all();
-    if (a.sel) {
-        a.parts = p.parts;
-        const int64_t tiles = ((int64_t)a.q_block * G + 31) / 32 * a.NQ;
-        if (launch_few<T, D, kSelected>(st, a, tiles, a.B)) return -1;
-    } else {
-        if (p.apart) {
-            a.parts = p.pre_parts;
-            if (launch_few<T, D, kAllRows>(st, a, ((int64_t)a.Mq * G + 31) / 32, 1)) return -1;
-            a.part0 = p.pre_parts;
-            a.pre = {};
-        }
-        a.parts = p.parts;
-        if (launch_few<T, D, kOwnRows>(st, a, ((int64_t)a.max_q * G + 31) / 32, a.B)) return -1;
+    if (a.all_parts > 1) {
+        a.part_o = (float *)workspace;
+        a.part_ml = a.part_o + (size_t)a.all_parts * a.Mq * a.H * D;
     }
-    if (!p.merged()) return 0;
+    if (p.apart) {
+        a.mode = kAllRows;
+        if (launch_rows<T, D>(st, a, p.pre, 1)) return -1;
+        a.part0 = p.pre.parts;
+        a.pre = {};
+    }
+    a.mode = a.sel ? kSelected : kOwnRows;
+    if (launch_rows<T, D>(st, a, p.rows, a.B)) return -1;
+    if (a.all_parts == 1) return 0;
     hipLaunchKernelGGL((k_keys_merge<T, D>), dim3((unsigned)(((int64_t)a.max_q * a.H + 3) / 4), 1, a.B), dim3(256), 0, st, a);
     return check_hip(hipGetLastError(), "attention merge launch");
 }
@@ -466,10 +787,10 @@ static bool sizes_fit(int Mq, int B, int max_q, int max_k, int H, int KV, int D)
 }
 
 static int check_keys(const char *who, const char *what, const KeySet &s, int KV, int D) {
-    if (s.rows < 0 || (s.rows && (!s.k || !s.vt || !aligned16(s.k) || (uintptr_t)s.vt % 2 || s.ldk < (int64_t)KV * D ||
+    if (s.rows < 0 || (s.rows && (!s.k || !s.vt || !aligned16(s.k) || (uintptr_t)s.vt % (s.ldv % 8 ? 2 : 16) || s.ldk < (int64_t)KV * D ||
                                   s.ldk % 8 || s.ldv < s.rows || s.ldk > (1LL << 28) || s.ldv > (1LL << 31)))) {
         set_error("%s: %s need 16-byte aligned k rows of a pitch >= KV * D in multiples of 8 and transposed v of a pitch >= "
-                  "rows (rows=%d ldk=%lld ldv=%lld)", who, what, s.rows, (long long)s.ldk, (long long)s.ldv);
+                  "rows, 16-byte aligned where that is a multiple of 8 (rows=%d ldk=%lld ldv=%lld)", who, what, s.rows, (long long)s.ldk, (long long)s.ldv);
         return -1;
     }
     return 0;
@@ -511,9 +832,10 @@ static int check_workspace(const char *who, size_t need, const void *ws, size_t 
 
 using namespace e2mi;
 
-extern "C" size_t e2mi_attention_prefix_workspace_bytes(int Mq, int P, int B, int max_q, int max_k, int H, int KV, int D) {
-    if (!sizes_fit(Mq, B, max_q, max_k, H, KV, D) || P < 0 || !Mq || !B || !max_q) return 0;
-    return part_bytes(plan_prefix(Mq, P, B, max_q, max_k, H, KV), Mq, H, D);
+extern "C" size_t e2mi_attention_prefix_workspace_bytes(int Mq, int Mk, int64_t ldv, int P, int64_t ldpv, int B, int max_q, int max_k,
+                                                        int H, int KV, int D) {
+    if (!sizes_fit(Mq, B, max_q, max_k, H, KV, D) || Mk < 0 || P < 0 || !Mq || !B || !max_q) return 0;
+    return workspace_of(plan_prefix(Mq, {nullptr, nullptr, 0, ldv, Mk}, {nullptr, nullptr, 0, ldpv, P}, B, max_q, max_k, H, KV, D), Mq, H, D);
 }
 
 extern "C" int e2mi_attention_prefix(e2mi_stream stream, int dtype, const uint16_t *q, int64_t ldq, int Mq, const uint16_t *k,
@@ -534,14 +856,16 @@ extern "C" int e2mi_attention_prefix(e2mi_stream stream, int dtype, const uint16
     if (check_call("attention_prefix", dtype, a, D, scale)) return -1;
     if (check_keys("attention_prefix", "prefix keys", a.pre, KV, D)) return -1;
     if (!Mq || !B || !max_q) return 0;
-    const KeysPlan p = plan_prefix(Mq, P, B, max_q, max_k, H, KV);
-    if (check_workspace("attention_prefix", part_bytes(p, Mq, H, D), workspace, workspace_bytes)) return -1;
+    const KeysPlan p = plan_prefix(Mq, a.own, a.pre, B, max_q, max_k, H, KV, D);
+    if (check_workspace("attention_prefix", workspace_of(p, Mq, H, D), workspace, workspace_bytes)) return -1;
     return run_keys((hipStream_t)stream, dtype, D, a, p, workspace);
 }
 
-extern "C" size_t e2mi_attention_blocks_workspace_bytes(int Mq, int B, int max_q, int H, int KV, int D, int q_block, int n_sel) {
-    if (!sizes_fit(Mq, B, max_q, 0, H, KV, D) || q_block <= 0 || n_sel <= 0 || n_sel > kMaxSelect || !Mq || !B || !max_q) return 0;
-    return part_bytes(plan_blocks(B, max_q, H, KV, q_block, n_sel), Mq, H, D);
+extern "C" size_t e2mi_attention_blocks_workspace_bytes(int Mq, int Mk, int64_t ldv, int B, int max_q, int H, int KV, int D, int q_block,
+                                                        int n_sel) {
+    if (!sizes_fit(Mq, B, max_q, 0, H, KV, D) || Mk < 0 || q_block <= 0 || n_sel <= 0 || n_sel > kMaxSelect || !Mq || !B || !max_q)
+        return 0;
+    return workspace_of(plan_blocks({nullptr, nullptr, 0, ldv, Mk}, B, max_q, H, KV, D, q_block, n_sel), Mq, H, D);
 }
 
 extern "C" int e2mi_attention_blocks(e2mi_stream stream, int dtype, const uint16_t *q, int64_t ldq, int Mq, const uint16_t *k,
@@ -566,7 +890,7 @@ extern "C" int e2mi_attention_blocks(e2mi_stream stream, int dtype, const uint16
     }
     if (!Mq || !B || !max_q) return 0;
     a.NQ = (max_q + q_block - 1) / q_block;
-    const KeysPlan p = plan_blocks(B, max_q, H, KV, q_block, n_sel);
-    if (check_workspace("attention_blocks", part_bytes(p, Mq, H, D), workspace, workspace_bytes)) return -1;
+    const KeysPlan p = plan_blocks(a.own, B, max_q, H, KV, D, q_block, n_sel);
+    if (check_workspace("attention_blocks", workspace_of(p, Mq, H, D), workspace, workspace_bytes)) return -1;
     return run_keys((hipStream_t)stream, dtype, D, a, p, workspace);
 }

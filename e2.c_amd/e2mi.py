@@ -97,14 +97,14 @@ SIGNATURES = {
     "e2mi_gather_ids": (_I, [_P, _P, _P, _I, _P]),
     "e2mi_rope_freqs": (_I, [_P, _I, _D, _I, _D, _I, _D, _D]),
     "e2mi_rope": (_I, [_P, _I, _I, _I, _P, _L, _P, _L, _I, _P, _L, _P, _L, _I, _I, _I, _P, _P, _I, _F]),
-    "e2mi_attention_prefix_workspace_bytes": (C.c_size_t, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "e2mi_attention_prefix_workspace_bytes": (C.c_size_t, [_I, _I, _L, _I, _L, _I, _I, _I, _I, _I, _I]),
     "e2mi_attention_prefix": (_I, [_P, _I, _P, _L, _I, _P, _L, _P, _L, _I, _P, _L, _P, _L, _I, _P, _P, _P, _P, _I, _I, _I,
                                    _I, _I, _I, _F, _I, _P, _L, _P, _P, _P, C.c_size_t]),
     "e2mi_block_bounds": (_I, [_P, _I, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
     "e2mi_block_select_workspace_bytes": (C.c_size_t, [_I, _I, _I, _I, _I]),
     "e2mi_block_select": (_I, [_P, _I, _P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P,
                                C.c_size_t]),
-    "e2mi_attention_blocks_workspace_bytes": (C.c_size_t, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "e2mi_attention_blocks_workspace_bytes": (C.c_size_t, [_I, _I, _L, _I, _I, _I, _I, _I, _I, _I]),
     "e2mi_attention_blocks": (_I, [_P, _I, _P, _L, _I, _P, _L, _P, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P,
                                    _I, _F, _I, _P, _L, _P, _P, _P, C.c_size_t]),
     # backend-selection surface (include/e2_dispatch.h)
@@ -896,7 +896,7 @@ def attention_prefix(q, k, vt, pk, pvt, q_start, q_len, max_q, H, KV, k_start=No
     _i32(q.device, B, q_start=q_start, q_len=q_len, k_start=k_start, k_len=k_len)
     own, pre = _keys_of("attention_prefix", k, vt, KV, D), _keys_of("attention_prefix", pk, pvt, KV, D)
     ctx, cq, cs = _contexts("attention_prefix", q, H, D, ctx, quant, stream)
-    ws, wp, wn = _workspace(lib.e2mi_attention_prefix_workspace_bytes(Mq, pre[4], B, max_q, max_k, H, KV, D), workspace, q.device,
+    ws, wp, wn = _workspace(lib.e2mi_attention_prefix_workspace_bytes(Mq, own[4], own[3], pre[4], pre[3], B, max_q, max_k, H, KV, D), workspace, q.device,
                             stream)
     check(lib.e2mi_attention_prefix(_stream(stream), kind, _p(q), _ld(q, H * D), Mq, *own, *pre, _p(q_start), _p(q_len),
                                     _p(k_start), _p(k_len), B, max_q, max_k, H, KV, D, scale, int(causal), _p(ctx),
@@ -967,7 +967,7 @@ def attention_blocks(q, k, vt, sel, q_start, q_len, k_start, k_len, max_q, max_k
     own = _keys_of("attention_blocks", k, vt, KV, D)
     ctx, cq, cs = _contexts("attention_blocks", q, H, D, ctx, quant, stream)
     n_sel = sel.shape[3]
-    ws, wp, wn = _workspace(lib.e2mi_attention_blocks_workspace_bytes(Mq, B, max_q, H, KV, D, q_block, n_sel), workspace, dev,
+    ws, wp, wn = _workspace(lib.e2mi_attention_blocks_workspace_bytes(Mq, own[4], own[3], B, max_q, H, KV, D, q_block, n_sel), workspace, dev,
                             stream)
     check(lib.e2mi_attention_blocks(_stream(stream), kind, _p(q), _ld(q, H * D), Mq, *own, _p(q_start), _p(q_len), _p(k_start),
                                     _p(k_len), B, max_q, max_k, H, KV, D, q_block, _p(sel), n_sel, scale, int(causal), _p(ctx),

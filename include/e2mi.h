@@ -382,8 +382,8 @@ int e2mi_rope(e2mi_stream stream, int dtype, int layout, int inverse, const void
  * [k_start[b], k_start[b] + k_len[b]) of Mk (rows of K, columns of V^T; every k_start a multiple of 8; q and
  * k ranges may be the same arrays), q_len[b] <= max_q and k_len[b] <= max_k: a longer range is cut, one
  * outside the rows given or off a multiple of 8 reads as empty. Rows of q are [H][D], of k [KV][D], head h
- * reads kv head h / (H / KV), vt is [KV][D][ldv] (any pitch of at least its rows); D 64, 128, 256 or 512;
- * dtype E2MI_F16 or E2MI_BF16 (bits in uint16_t); pitches in elements, those of rows multiples of 8, rows
+ * reads kv head h / (H / KV), vt is [KV][D][ldv] (any pitch of at least its rows, 16-byte aligned where
+ * that is a multiple of 8); D 64, 128, 256 or 512; dtype E2MI_F16 or E2MI_BF16 (bits in uint16_t); pitches in elements, those of rows multiples of 8, rows
  * 16-byte aligned. causal: query i of a sequence reads its own keys j <= i + k_len - q_len (the ends aligned). A row
  * that sees no key gets a context of 0; rows outside every sequence are not written, and no value outside a
  * sequence's keys (of any bits) changes a result. Softmax and sums are f32. The context goes to ctx [Mq][H][D]
@@ -395,7 +395,8 @@ int e2mi_rope(e2mi_stream stream, int dtype, int layout, int inverse, const void
  * keys subject to causal. Positions are in the rows (turned by the caller; e2mi_rope). The prefix's keys are
  * kept once; sequences of a few rows are also computed against it together, a pass over its keys for all, its
  * key range shared out over the device where rows are few. P or Mk may be 0. */
-size_t e2mi_attention_prefix_workspace_bytes(int Mq, int P, int B, int max_q, int max_k, int H, int KV, int D);
+size_t e2mi_attention_prefix_workspace_bytes(int Mq, int Mk, int64_t ldv, int P, int64_t ldpv, int B, int max_q,
+                                             int max_k, int H, int KV, int D);
 int e2mi_attention_prefix(e2mi_stream stream, int dtype, const uint16_t *q, int64_t ldq, int Mq,
                           const uint16_t *k, int64_t ldk, const uint16_t *vt, int64_t ldv, int Mk,
                           const uint16_t *pk, int64_t ldpk, const uint16_t *pvt, int64_t ldpv, int P,
@@ -432,8 +433,8 @@ int e2mi_block_select(e2mi_stream stream, int dtype, const uint16_t *q, int64_t 
  * sequence: its tokens [i * q_block, (i + 1) * q_block)): sel [B][ceil(max_q / q_block)][KV][n_sel], n_sel <=
  * 2048, q_block <= 1024; entries below 0 or past the sequence's last block are passed over, an entry that is
  * listed twice counts its keys twice. */
-size_t e2mi_attention_blocks_workspace_bytes(int Mq, int B, int max_q, int H, int KV, int D, int q_block,
-                                             int n_sel);
+size_t e2mi_attention_blocks_workspace_bytes(int Mq, int Mk, int64_t ldv, int B, int max_q, int H, int KV, int D,
+                                             int q_block, int n_sel);
 int e2mi_attention_blocks(e2mi_stream stream, int dtype, const uint16_t *q, int64_t ldq, int Mq,
                           const uint16_t *k, int64_t ldk, const uint16_t *vt, int64_t ldv, int Mk,
                           const int32_t *q_start, const int32_t *q_len, const int32_t *k_start,

@@ -17,7 +17,7 @@ NOTHING = dict(B=0)  # what is checked, and then has nothing to do
 ROWS = [dict(dtype=2), dict(dtype=-1), dict(Mq=-1), dict(B=-1), dict(B=65536), dict(max_q=-1), dict(max_k=-1), dict(H=0), dict(KV=0),
         dict(KV=2), dict(D=96), dict(D=0), dict(q=None), dict(q=X + 8), dict(ldq=767), dict(ldq=772), dict(ldq=1 << 40), dict(qs=None),
         dict(ql=None), dict(kl=None)]
-KEYS = [dict(k=None), dict(k=2 * X + 2), dict(ldk=255), dict(ldk=260), dict(vt=None), dict(vt=3 * X + 1), dict(ldv=63), dict(Mk=-1),
+KEYS = [dict(k=None), dict(k=2 * X + 2), dict(ldk=255), dict(ldk=260), dict(vt=None), dict(vt=3 * X + 1), dict(vt=3 * X + 2), dict(ldv=63), dict(Mk=-1),
         dict(ks=None)]
 OUT = [dict(ctx=None), dict(ctx=10 * X + 4), dict(ldc=760), dict(ldc=770), dict(cq=X), dict(cs=X), dict(ctx=None, cq=X), dict(cq=X + 4, cs=X),
        dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan"))]
@@ -75,11 +75,11 @@ def test_workspace_sizes():
     import e2mi
     lib = e2mi.load()
     size = lib.e2mi_attention_prefix_workspace_bytes
-    assert size(64, 33, 2, 32, 32, 3, 1, 96) == 0 and size(64, -1, 2, 32, 32, 3, 1, 256) == 0
-    assert lib.e2mi_attention_blocks_workspace_bytes(64, 2, 32, 3, 1, 256, 0, 4) == 0
+    assert size(64, 64, 64, 33, 33, 2, 32, 32, 3, 1, 96) == 0 and size(64, 64, 64, -1, 33, 2, 32, 32, 3, 1, 256) == 0
+    assert lib.e2mi_attention_blocks_workspace_bytes(64, 64, 64, 2, 32, 3, 1, 256, 0, 4) == 0
     assert lib.e2mi_block_select_workspace_bytes(2, 32, 640, 1, 16) == 2 * 2 * 10 * 4
     few = dict(PREFIX, Mq=1, B=1, max_q=1, P=4096, ldpv=4096)
-    need = size(1, 4096, 1, 1, 32, 3, 1, 256)
+    need = size(1, 64, 64, 4096, 4096, 1, 1, 32, 3, 1, 256)
     assert need >= 2 * 3 * (256 + 2) * 4
     for over in (dict(ws=None, wn=0), dict(wn=need - 1), dict(ws=X + 4)):
         assert lib.e2mi_attention_prefix(*{**few, **over}.values()) == -1
