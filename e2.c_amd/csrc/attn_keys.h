@@ -6,7 +6,7 @@
 namespace e2mi {
 
 constexpr int kKeyBlock = E2MI_KEY_BLOCK;  // keys of a selectable block
-constexpr int kMaxKeyParts = 64;           // shares of a key range, merged by one wave's lanes
+constexpr int kMaxKeyParts = 128;          // shares of a key range, two a lane of the wave that joins them
 constexpr int kMaxSelect = 2048;           // entries of a selection list
 
 // Keys of a call: rows [rows][ldk] of K (kv heads side by side) and V transposed, [KV * D][ldv].

@@ -214,127 +214,201 @@ __device__ __forceinline__ void write_share(const KeysArgs &a, const f16v (&o)[D
             *(float4 *)(y + 32 * i + 8 * g) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
 }
 
-// Few rows: 32 a workgroup, whose four waves take every fourth key tile and are joined through LDS. Fragments
-// go from global memory to registers: a tile's K and V^T are read by one wave only, so LDS would hold them for
-// nobody else, and the reads in flight are bounded by registers, not by LDS.
+// Few rows: 16 a workgroup, whose four waves take every fourth key tile and are joined through LDS. Fragments go from
+// global memory to registers: a tile's K and V^T are read by one wave only, so LDS would hold them for nobody else.
+// Bound by HBM, hence by what is in flight: a wave's next K tile is requested when its logits are done, the next V^T
+// tile when its context is, 16 KB each at head_dim 256.
+//
+// 16x16x32 MFMA: half the registers of the 32-row form for Q and the context, which is what lets the tiles in flight
+// fit. Logits of 32 keys are two products whose K rows are permuted (row 4 g + i of product u holds key 8 g + 4 u + i)
+// so that a lane ends with 8 consecutive keys of one row, the operand of the next product.
+typedef float f4v __attribute__((ext_vector_type(4)));
+template <class T>
+__device__ inline f4v mma16(typename Half8<T>::type a, typename Half8<T>::type b, f4v c) {
+    if constexpr (sizeof(T) == 2 && __is_same(T, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+template <int D>
+constexpr size_t few_lds() { return 4 * 16 * (D + 4) * 4; }
+
 template <class T, int D>
-__global__ __launch_bounds__(256, D == 512 ? 1 : 2) void k_keys_few(KeysArgs a) {
+__global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) {
     typedef typename Half8<T>::type V8;
-    constexpr int NQ = D / 16, NO = D / 32;
-    extern __shared__ __align__(16) float few_smem[];  // the list (kSelected), then two waves' o (join)
-    __shared__ float s_m[4][32], s_l[4][32];
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    // V^T tiles held at once: at head_dim 512 half of them (all would spill), requested as the tile comes up
+    constexpr int NQ = D / 32, NO = D / 16, PITCH = D + 4, NP = D == 512 ? 2 : 1, NV = NO / NP;
+    extern __shared__ __align__(16) float few_smem[];  // the waves' contexts [4][16][PITCH], then the list (kSelected)
+    __shared__ float s_m[4][16], s_l[4][16];
     __shared__ int s_count;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5;
-    int *list = (int *)few_smem;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, g = lane >> 4;
+    int *list = (int *)(few_smem + 4 * 16 * PITCH);
     Walk k;
-    if (!start_walk<32>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
+    if (!start_walk<16>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
                         &s_count, k))
         return;
-    const int r = k.r0 + (lane & 31), rc = min(r, k.rows - 1);
-    const int tok = k.tok0 + rc / a.G, h = k.kvh * a.G + rc % a.G;
-    const int64_t m = (int64_t)k.qs + tok;
-    const int last = a.causal ? min(tok + k.back, k.nk - 1) : k.nk - 1;  // own keys this row sees
-
+    int last;  // own keys this lane's row sees
     V8 qf[NQ];
     {
-        const uint16_t *qp = a.q + m * a.ldq + (int64_t)h * D + 8 * half;
+        const int r = min(k.r0 + c, k.rows - 1), tok = k.tok0 + r / a.G, h = k.kvh * a.G + r % a.G;
+        last = a.causal ? min(tok + k.back, k.nk - 1) : k.nk - 1;
+        const uint16_t *qp = a.q + ((int64_t)k.qs + tok) * a.ldq + (int64_t)h * D + 8 * g;
 #pragma unroll
-        for (int s = 0; s < NQ; s++) qf[s] = *(const V8 *)(qp + 16 * s);
+        for (int s = 0; s < NQ; s++) qf[s] = *(const V8 *)(qp + 32 * s);
     }
-    f16v o[NO];
+    f4v o[NO];
 #pragma unroll
-    for (int t = 0; t < NO; t++) o[t] = (f16v){};
+    for (int t = 0; t < NO; t++) o[t] = (f4v){};
     float mrun = -INFINITY, lrun = 0.f;
 
-    for (int t = k.t0 + w; t < k.t1; t += 4) {
-        const KeyTile kt = key_tile(a, k, list, t);
-        if (kt.n <= 0) continue;
+    // tile t: where its keys lie; one without keys (the second half of a short last block) reads the first key and counts none
+    auto place = [&](int t) {
+        KeyTile kt = key_tile(a, k, list, t);
+        if (kt.n <= 0) kt.n = 0, kt.key0 = 0;
+        return kt;
+    };
+    V8 kf[2][NQ], vf[NV];
+    auto load_k = [&](const KeyTile &kt) {
         const KeySet &src = kt.pre ? a.pre : a.own;
         const int64_t row = (kt.pre ? 0 : k.ks) + kt.key0;
-        const uint16_t *kp = src.k + (row + min(swap23(lane & 31), kt.n - 1)) * src.ldk + (int64_t)k.kvh * D + 8 * half;
-        f16v st = (f16v){};
 #pragma unroll
-        for (int s = 0; s < NQ; s++) st = Half8<T>::mma(*(const V8 *)(kp + 16 * s), qf[s], st);
-        float tv[16];
+        for (int u = 0; u < 2; u++) {
+            const int key = max(0, min(8 * (c >> 2) + 4 * u + (c & 3), kt.n - 1));
+            const uint16_t *kp = src.k + (row + key) * src.ldk + (int64_t)k.kvh * D + 8 * g;
 #pragma unroll
-        for (int i = 0; i < 16; i++) tv[i] = st[i];
-        if (kt.n < 32 || (!kt.pre && a.causal)) {
-            const int top = kt.pre ? kt.n - 1 : min(last - kt.key0, kt.n - 1);
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (16 * (i >> 3) + 8 * half + (i & 7) > top) tv[i] = -INFINITY;
+            for (int s = 0; s < NQ; s++) kf[u][s] = *(const V8 *)(kp + 32 * s);
         }
-        V8 pb[2];
-        const float alpha = softmax_step<T>(tv, a.c2, mrun, lrun, pb);
-        if (__any(alpha != 1.f)) {
-#pragma unroll
-            for (int i = 0; i < NO; i++) o[i] *= alpha;
-        }
-        const uint16_t *vp = src.vt + ((int64_t)k.kvh * D + (lane & 31)) * src.ldv + row + 8 * half;
+    };
+    auto load_v = [&](const KeyTile &kt, int piece) {
+        const KeySet &src = kt.pre ? a.pre : a.own;
+        const uint16_t *vp = src.vt + ((int64_t)k.kvh * D + piece * (D / NP) + c) * src.ldv + (kt.pre ? 0 : k.ks) + kt.key0 + 8 * g;
         if (kt.n == 32) {
 #pragma unroll
-            for (int i = 0; i < 2 * NO; i++)
-                o[i >> 1] = Half8<T>::mma(load8<T>(vp + (int64_t)(i >> 1) * 32 * src.ldv + 16 * (i & 1)), pb[i & 1], o[i >> 1]);
+            for (int t = 0; t < NV; t++) vf[t] = load8<T>(vp + (int64_t)t * 16 * src.ldv);
         } else {
-            // values past the range are not read (they may lie past the tensor) and count as 0: a zero
-            // probability times an infinity would be a NaN
-            const int left = kt.n - 8 * half;
-            for (int i = 0; i < 2 * NO; i++) {
-                const int have = left - 16 * (i & 1);
-                const uint16_t *x = vp + (int64_t)(i >> 1) * 32 * src.ldv + 16 * (i & 1);
-                V8 vf = {};
+            // values past the range are not read (they may lie past the tensor) and count as 0: a zero probability
+            // times an infinity would be a NaN
+            const int have = kt.n - 8 * g;
+#pragma unroll
+            for (int t = 0; t < NV; t++) {
+                const uint16_t *x = vp + (int64_t)t * 16 * src.ldv;
+                V8 v = {};
                 if (have >= 8) {
-                    vf = load8<T>(x);
+                    v = load8<T>(x);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 7; e++)
-                        if (e < have) vf[e] = __builtin_bit_cast(T, x[e]);
+                        if (e < have) v[e] = __builtin_bit_cast(T, x[e]);
                 }
-#pragma unroll
-                for (int u = 0; u < NO; u++)
-                    if (u == i >> 1) o[u] = Half8<T>::mma(vf, pb[i & 1], o[u]);
+                vf[t] = v;
             }
+        }
+    };
+    KeyTile now = {}, next = {};
+    if (k.t0 + w < k.t1) {
+        now = place(k.t0 + w);
+        load_k(now);
+        if (NP == 1) load_v(now, 0);
+    }
+    for (int t = k.t0 + w; t < k.t1; t += 4, now = next) {
+        const bool more = t + 4 < k.t1;
+        if (NP > 1) load_v(now, 0);
+        f4v st[2] = {};
+#pragma unroll
+        for (int s = 0; s < NQ; s++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) st[u] = mma16<T>(kf[u][s], qf[s], st[u]);
+        if (more) {
+            next = place(t + 4);
+            load_k(next);
+        }
+        float tv[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) tv[i] = st[i >> 2][i & 3];
+        if (now.n < 32 || (!now.pre && a.causal)) {
+            const int top = now.pre ? now.n - 1 : min(last - now.key0, now.n - 1);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (8 * g + i > top) tv[i] = -INFINITY;
+        }
+        float mloc = tv[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) mloc = fmaxf(mloc, tv[i]);
+        mloc = fmaxf(mloc, xor_lane<16>(mloc));
+        mloc = fmaxf(mloc, xor_lane<32>(mloc));
+        const float mc = mloc * a.c2;
+        if (mc > mrun + kTau) {
+            const float alpha = __builtin_amdgcn_exp2f(mrun - mc);
+            mrun = mc;
+            lrun *= alpha;
+#pragma unroll
+            for (int i = 0; i < NO; i++) o[i] *= alpha;
+        }
+        const float ms = mrun == -INFINITY ? 0.f : mrun;
+        V8 pb;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(tv[i], a.c2, -ms));
+            lrun += p;
+            pb[i] = (T)p;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) o[i] = mma16<T>(vf[i], pb, o[i]);
+        if constexpr (NP > 1) {
+            load_v(now, 1);
+#pragma unroll
+            for (int i = 0; i < NV; i++) o[NV + i] = mma16<T>(vf[i], pb, o[NV + i]);
+        } else if (more) {
+            load_v(next, 0);
         }
     }
 
-    // join the four waves: a common maximum, then two by two through LDS
-    float lsum = lrun + xor_lane<32>(lrun);
-    if (half == 0) s_m[w][lane] = mrun, s_l[w][lane] = lsum;
-    __syncthreads();  // the list is no longer read
-    const int c = lane & 31;
-    const float mall = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c]));
-    auto share = [&](float mp) { return mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mall); };
-    lsum = 0.f;
+    // join the four waves: contexts as they are, with their maxima and sums; a quad of dims a thread
+    float lsum = lrun + xor_lane<16>(lrun);
+    lsum += xor_lane<32>(lsum);
+    if (g == 0) s_m[w][c] = mrun, s_l[w][c] = lsum;
+    {
+        float *y = few_smem + (w * 16 + c) * PITCH + 4 * g;
 #pragma unroll
-    for (int i = 0; i < 4; i++) lsum += s_l[i][c] * share(s_m[i][c]);
-    const float mine = share(mrun);
-#pragma unroll
-    for (int i = 0; i < NO; i++) o[i] *= mine;
-    constexpr int kWave = NO * 16 * 64;  // floats of one wave's o
-#pragma unroll
-    for (int step = 2; step > 0; step >>= 1) {
-        if (w >= step && w < 2 * step) {
-            float *buf = few_smem + (w - step) * kWave + lane;
-#pragma unroll
-            for (int i = 0; i < NO * 16; i++) buf[i * 64] = o[i >> 4][i & 15];
-        }
-        __syncthreads();
-        if (w < step) {
-            const float *buf = few_smem + w * kWave + lane;
-#pragma unroll
-            for (int i = 0; i < NO * 16; i++) o[i >> 4][i & 15] += buf[i * 64];
-        }
-        if (step > 1) __syncthreads();
+        for (int i = 0; i < NO; i++) *(f4v *)(y + 16 * i) = o[i];
     }
-    if (w || r >= k.rows) return;
-    if (a.part_o) {
-        write_share<D>(a, o, mall, lsum, k.part, m, h, half);
-        return;
-    }
-    const float inv = lsum == 0.f ? 0.f : __fdiv_rn(1.f, lsum);
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NO; i++) o[i] *= inv;
-    write_row<T, D>(a, o, m, h, half);
+    for (int i = 0; i < D / 64; i++) {
+        const int at = tid + 256 * i, row = at / (D / 4), d = at % (D / 4) * 4, r = k.r0 + row;
+        const float mall = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+        f4v v = {};
+        float sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const float mx = s_m[x][row], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mall);
+            v += *(const f4v *)(few_smem + (x * 16 + row) * PITCH + d) * f;
+            sum += s_l[x][row] * f;
+        }
+        if (sum != sum) v = (f4v)NAN;
+        const bool live = r < k.rows;
+        const int rc = live ? r : k.rows - 1, h = k.kvh * a.G + rc % a.G;
+        const int64_t m = (int64_t)k.qs + k.tok0 + rc / a.G;
+        if (a.part_o) {
+            const int64_t to = ((int64_t)(a.part0 + k.part) * a.Mq + m) * a.H + h;
+            if (live && d == 0) *(float2 *)(a.part_ml + to * 2) = make_float2(sum == sum ? mall : INFINITY, sum);
+            if (live && sum != 0.f) *(f4v *)(a.part_o + to * D + d) = v;
+            continue;
+        }
+        v *= sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+        if (a.ctx && live) {
+            const T4 y = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+            *(T4 *)((T *)a.ctx + m * a.ldc + (int64_t)h * D + d) = y;
+        }
+        if constexpr (D % 128 == 0) {
+            if (a.cq) {  // 128 dims: 32 lanes
+                const QScale q = qscale(group_max<32>(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))));
+                if (live) {
+                    *(uint32_t *)(a.cq + (m * a.H + h) * D + d) = pack4_magic(v[0], v[1], v[2], v[3], q.inv);
+                    if (d % 128 == 0) a.cs[(m * a.H + h) * (D / 128) + d / 128] = q.sc;
+                }
+            }
+        }
+    }
 }
 
 // Many rows: 32 a row group, NW groups that share the key tiles in LDS, fetched one tile ahead by direct-to-LDS
@@ -580,7 +654,8 @@ __global__ __launch_bounds__(256) void k_pad_rows(uint16_t *y, int64_t ldy, cons
     }
 }
 
-// Joins the shares of a row: a wave a row, lane p holding share p's maximum and sum, then D / 64 dims a lane.
+// Joins the shares of a row: a wave a row, lane p holding the maxima and sums of shares p and p + 64, then D / 64 dims a
+// lane, eight shares' contexts in flight.
 template <class T, int D>
 __global__ __launch_bounds__(256) void k_keys_merge(KeysArgs a) {
     constexpr int VW = D / 64;
@@ -592,20 +667,36 @@ __global__ __launch_bounds__(256) void k_keys_merge(KeysArgs a) {
     const int64_t i = (int64_t)blockIdx.x * 4 + w;
     if (i >= (int64_t)nq * a.H) return;
     const int64_t row = (int64_t)qs * a.H + i, pitch = (int64_t)a.Mq * a.H;
-    float mp = -INFINITY, lp = 0.f;
-    if (lane < a.all_parts) {
-        const float2 ml = *(const float2 *)(a.part_ml + (lane * pitch + row) * 2);
-        mp = ml.x, lp = ml.y;
+    float mp[2], wp[2], sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        mp[x] = -INFINITY, wp[x] = 0.f;
+        if (lane + 64 * x < a.all_parts) {
+            const float2 ml = *(const float2 *)(a.part_ml + ((lane + 64 * x) * pitch + row) * 2);
+            mp[x] = ml.x, wp[x] = ml.y;
+        }
     }
-    const float mall = group_max<64>(mp);
-    const float wp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mall);
-    const float sum = group_sum<64>(wp * lp);
+    const float mall = group_max<64>(fmaxf(mp[0], mp[1]));
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const float f = mp[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp[x] - mall);
+        sum += f * wp[x];
+        wp[x] = wp[x] == 0.f ? 0.f : f;  // a share without keys left no context
+    }
+    sum = group_sum<64>(sum);
     vf o = {};
-    for (int p = 0; p < a.all_parts; p++) {
-        const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wp), p));
-        if (__builtin_bit_cast(int, f) == 0) continue;  // a share without keys left no o
-        const vf v = *(const vf *)(a.part_o + (p * pitch + row) * D + lane * VW);
-        o += v * f;
+    const float *from = a.part_o + row * D + lane * VW;
+    for (int p0 = 0; p0 < a.all_parts; p0 += 8) {
+        vf v[8];
+#pragma unroll
+        for (int x = 0; x < 8; x++) v[x] = *(const vf *)(from + min(p0 + x, a.all_parts - 1) * pitch * D);
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+            const int p = p0 + x;
+            const float f = __builtin_bit_cast(float, p < 64 ? __builtin_amdgcn_readlane(__builtin_bit_cast(int, wp[0]), p & 63)
+                                                             : __builtin_amdgcn_readlane(__builtin_bit_cast(int, wp[1]), p & 63));
+            if (p < a.all_parts && f != 0.f) o += v[x] * f;
+        }
     }
     const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
     o *= inv;
@@ -662,7 +753,7 @@ static int key_shares(int64_t groups, int64_t tiles, int least, int most) {
 static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int most, bool wide) {
     RowsPlan p;
     p.nw = !wide || rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
-    const int R = p.nw ? 32 * p.nw : 32;
+    const int R = p.nw ? 32 * p.nw : 16;
     p.tiles = (rows + R - 1) / R;
     p.parts = key_shares(p.tiles * count, tiles, 8, most);
     return p;
@@ -725,9 +816,9 @@ static int launch_rows(hipStream_t st, KeysArgs a, const RowsPlan &p, int B) {
     if (p.nw == 2) return launch_wide<T, D, 2>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 3) return launch_wide<T, D, 3>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 4) return launch_wide<T, D, 4>(st, a, p.tiles, grid * a.KV * B);
-    const size_t list = a.mode == kSelected ? 4 * (size_t)a.n_sel : 0, join = (size_t)D * 256, lds = list > join ? list : join;
-    if (lds > 65536 && check_hip(hipFuncSetAttribute((const void *)k_keys_few<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                     (int)lds), "lds attribute"))
+    const size_t lds = few_lds<D>() + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
+    if (check_hip(hipFuncSetAttribute((const void *)k_keys_few<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
+                  "lds attribute"))
         return -1;
     hipLaunchKernelGGL((k_keys_few<T, D>), dim3((unsigned)grid, a.KV, B), dim3(256), lds, st, a);
     return check_hip(hipGetLastError(), "attention launch");

@@ -100,107 +100,6 @@ struct SelectArgs {
     int32_t *sel;   // [B][NQ][KV][n_sel]
 };
 
-// Scores: a workgroup takes 32 / group query blocks (of up to 32 rows each; a query block of more rows takes
-// all 32, tile after tile) against its share of the blocks, a wave 32 blocks at a time.
-template <class T, int D>
-__global__ __launch_bounds__(256) void k_block_scores(SelectArgs a) {
-    constexpr int K2 = 2 * D, PITCH = K2 + 16;
-    __shared__ __align__(16) int8_t s_q[32 * PITCH];
-    __shared__ float s_sc[32];
-    __shared__ int s_last[32];  // last key a row sees (-1: none)
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5;
-    const int kvh = blockIdx.y, b = blockIdx.z;
-    const int per = 32 / a.group;
-    const int shares = (a.NB + 127) / 128;
-    const int share = (int)(blockIdx.x % (unsigned)shares), qb0 = (int)(blockIdx.x / (unsigned)shares) * per;
-    int qs, nq;
-    if (!row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, qs, nq)) return;
-    if ((int64_t)qb0 * a.q_block >= nq) return;
-    const int nk = max(0, min(a.k_len[b], a.max_k));
-    const int n0 = share * 128 + w * 32;  // this wave's blocks
-    const int n = n0 + (lane & 31);
-    const int R = a.q_block * a.G;  // rows of a query block
-    float best[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) best[i] = -INFINITY;
-    v4i bf[K2 / 32];
-    const bool some = n0 * kKeyBlock < nk;
-    if (some) {
-        const int64_t slot = ((int64_t)b * a.NB + min(n, (nk - 1) / kKeyBlock)) * a.KV + kvh;
-#pragma unroll
-        for (int s = 0; s < K2 / 32; s++) bf[s] = *(const v4i *)(a.bounds + slot * K2 + 32 * s + 16 * half);
-    }
-    for (int r0 = 0; r0 < (a.group == 32 ? R : 1); r0 += 32) {
-        if (r0) __syncthreads();
-        // quantize this tile's rows, a wave 8 of them
-        for (int i = w; i < 32; i += 4) {
-            const int blk = qb0 + i / a.group, in = r0 + i % a.group;
-            const int64_t tok = (int64_t)blk * a.q_block + in / a.G;
-            const bool row = in < R && tok < nq;
-            float x[D / 64];
-            float am = 0.f;
-            const uint16_t *qp = a.q + (qs + (row ? tok : 0)) * a.ldq + (int64_t)(kvh * a.G + in % a.G) * D;
-#pragma unroll
-            for (int e = 0; e < D / 64; e++) {
-                x[e] = row ? value_of<T>(qp[lane + 64 * e]) : 0.f;
-                am = fmaxf(am, fabsf(x[e]));
-            }
-            const QScale q = qscale(group_max<64>(am));
-#pragma unroll
-            for (int e = 0; e < D / 64; e++) {
-                const int v = qbyte(x[e], q.inv);
-                s_q[i * PITCH + lane + 64 * e] = (int8_t)(v > 0 ? v : 0);
-                s_q[i * PITCH + D + lane + 64 * e] = (int8_t)(v < 0 ? v : 0);
-            }
-            if (lane == 0) {
-                s_sc[i] = q.sc;
-                s_last[i] = !row ? -1 : a.causal ? (int)tok + nk - nq : nk - 1;
-            }
-        }
-        __syncthreads();
-        if (!some) continue;
-        v16i acc = {};
-#pragma unroll
-        for (int s = 0; s < K2 / 32; s++)
-            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const v4i *)(s_q + (lane & 31) * PITCH + 32 * s + 16 * half), bf[s], acc, 0, 0, 0);
-        // lane: block n; register r: row 8 (r / 4) + 4 half + r % 4; best[] holds runs of 4 rows
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int row = 8 * (r >> 2) + 4 * half + (r & 3);
-            const float v = n * kKeyBlock <= s_last[row] ? __fmul_rn((float)acc[r], s_sc[row]) : -INFINITY;
-            best[r >> 2] = fmaxf(best[r >> 2], v);
-        }
-    }
-    if (!some) return;
-    // runs of 4 rows: register i of half h is rows 8 i + 4 h .. + 3
-    float other[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) other[i] = xor_lane<32>(best[i]);
-    const float ks = n * kKeyBlock < nk ? a.kscale[((int64_t)b * a.NB + n) * a.KV + kvh] : 0.f;
-    auto put = [&](int blk, float v) {
-        if (n * kKeyBlock < nk && (int64_t)(qb0 + blk) * a.q_block < nq)
-            a.scores[(((int64_t)b * a.NQ + qb0 + blk) * a.KV + kvh) * a.NB + n] = __fmul_rn(v, ks);
-    };
-    if (a.group == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) put(2 * i + half, best[i]);
-        return;
-    }
-    if (half) return;
-    float run[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) run[i] = fmaxf(best[i], other[i]);  // rows 8 i .. 8 i + 7
-    if (a.group == 8) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) put(i, run[i]);
-    } else if (a.group == 16) {
-        put(0, fmaxf(run[0], run[1]));
-        put(1, fmaxf(run[2], run[3]));
-    } else {
-        put(0, fmaxf(fmaxf(run[0], run[1]), fmaxf(run[2], run[3])));
-    }
-}
-
 // An order-preserving unsigned key of a score; NaN (an infinite bound times 0) comes last of those that may be taken.
 __device__ inline uint32_t order_key(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
@@ -208,14 +107,216 @@ __device__ inline uint32_t order_key(float v) {
     const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
     return k < 1 ? 1 : k > 0xfffffffeu ? 0xfffffffeu : k;
 }
+// the score of a key, NaN for none
+__device__ inline float score_of(uint32_t k) {
+    return k <= 1 ? NAN : __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
 
-// The n_sel largest: the n_sel-th largest key by bisection of its 32 bits (counts by ballots over keys held in
-// registers), then everything above it and the first of its equals, in block order. W waves a list, RPL keys
-// a lane: key 64 (w RPL + j) + lane is register j of wave w.
+// Scores: a matrix product of rows (in registers, quantized there) with the blocks' bounds (32 at a time through
+// LDS, fetched one tile ahead), whose 32 x 32 results shrink to a maximum per query block and block.
+//
+// A wave holds 32 row slots. Query blocks of up to 32 rows take 4, 8, 16 or 32 of them (`group`), so a tile's maxima
+// are the wave's own; a query block of more rows takes `span` slots of 32, over the waves and over passes, and
+// its maxima meet in LDS (a maximum does not depend on the order). A slot without a row has a NaN scale, which a
+// maximum passes over.
+//
+// Bound by LDS reads and the int8 MFMA unit alike (64 D bytes, D / 2 cycles of LDS, for 2 D cycles of a SIMD), by
+// the launch for few rows. 65521 x 4 rows of 512 against 1024 blocks: one wave a 32-row tile with the rows in LDS
+// and the bounds read from L2 by every wave took 3650 us.
+__device__ inline int byte_lanes_negative(uint32_t x) {  // 0xff in every negative byte
+    const uint32_t m = (x >> 7) & 0x01010101u;
+    return (int)((m << 8) - m);
+}
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int shares, int groups) {
+    constexpr int NS = D / 32, TILE = 64 * D, RPI = 512 / D, LPR = D / 8, NLW = D / 64;
+    extern __shared__ __align__(16) unsigned char sc_smem[];  // two tiles of bounds, then the maxima (span > 1)
+    __shared__ int s_last[128];
+    __shared__ float s_scale[128];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wu = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int id = xcd_swizzle(blockIdx.x, gridDim.x);
+    const int share = id % shares;
+    id /= shares;
+    const int at = id % groups;
+    id /= groups;
+    const int kvh = id % a.KV, b = id / a.KV;
+    const int R = a.q_block * a.G, span = (R + 31) / 32;     // 32-row slots of a query block
+    const int per = 32 / a.group;                            // query blocks of a slot (span 1)
+    const int wg_blocks = span > 4 ? 1 : span > 1 ? 4 / span : 4 * per;  // query blocks of this workgroup
+    const int qb0 = at * wg_blocks;
+    int qs, nq;
+    if (!row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, qs, nq)) return;
+    if ((int64_t)qb0 * a.q_block >= nq) return;
+    const int nk = max(0, min(a.k_len[b], a.max_k));
+    const int nb = (nk + kKeyBlock - 1) / kKeyBlock, all = (nb + 31) / 32;  // blocks, tiles of them
+    const int t0 = (int)((int64_t)all * share / shares), t1 = (int)((int64_t)all * (share + 1) / shares);
+    if (t0 >= t1) return;
+    uint32_t *s_best = (uint32_t *)(sc_smem + 2 * TILE);  // [wg_blocks][32 (t1 - t0)]: order keys, 0: none
+    const int width = 32 * (t1 - t0);
+    if (span > 1)
+        for (int i = tid; i < width * wg_blocks; i += 256) s_best[i] = 0;
+
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_void *)sc_smem);
+    const int lr = lane / LPR, lc = lane % LPR;
+    const uint32_t ldb = (uint32_t)a.KV * 2 * D;
+    auto load = [&](int t, int buf) {  // bounds of blocks 32 t .. + 31; those past the last read as zero
+        const int n0 = 32 * t, have = min(32, nb - n0);
+        const v4u rs = rsrc_words(a.bounds + (((int64_t)b * a.NB + n0) * a.KV + kvh) * (2 * D), (uint32_t)(have - 1) * ldb + 2 * D);
+#pragma unroll
+        for (int j = 0; j < NLW; j++) {
+            const int r = RPI * (NLW * wu + j);
+            dma16(rs, __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(buf * TILE + r * 2 * D)),
+                  (uint32_t)(r + lr) * ldb + (uint32_t)((lc ^ ((r + lr) & 7)) << 4), 0);
+        }
+    };
+    const int passes = span > 4 ? (span + 3) / 4 : 1;
+    for (int pass = 0; pass < passes; pass++) {
+        // this wave's slot: query block `blk` (of the workgroup; span 1: its first), rows from r0 of it
+        const int blk = span > 4 ? 0 : span > 1 ? wu / span : per * wu;
+        const int r0 = span > 4 ? 32 * (4 * pass + wu) : span > 1 ? wu % span * 32 : 0;
+        const bool live = blk < wg_blocks && r0 < R && (int64_t)(qb0 + blk) * a.q_block < nq;
+        // quantize: lane (row, half) holds 16 values of every 32
+        v4i up[NS], down[NS];
+        {
+            const int slot = lane & 31, in = span > 1 ? r0 + slot : slot % a.group;
+            const int64_t tok = (int64_t)(qb0 + blk + (span > 1 ? 0 : slot / a.group)) * a.q_block + in / a.G;
+            const bool row = live && in < R && tok < nq && in / a.G < a.q_block;
+            const uint16_t *qp = a.q + (qs + (row ? tok : 0)) * a.ldq + (int64_t)(kvh * a.G + in % a.G) * D + 16 * half;
+            uint32_t raw[NS][8];
+            float am = 0.f;
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                *(uint4 *)raw[s] = *(const uint4 *)(qp + 32 * s);
+                *(uint4 *)(raw[s] + 4) = *(const uint4 *)(qp + 32 * s + 8);
+            }
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    am = fmaxf(am, fmaxf(fabsf(value_of<T>((uint16_t)raw[s][e])), fabsf(value_of<T>((uint16_t)(raw[s][e] >> 16)))));
+            am = fmaxf(am, xor_lane<32>(am));
+            const QScale q = qscale(am);
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t u = raw[s][2 * e], v = raw[s][2 * e + 1];
+                    const uint32_t x = pack4(qbyte(value_of<T>((uint16_t)u), q.inv), qbyte(value_of<T>((uint16_t)(u >> 16)), q.inv),
+                                             qbyte(value_of<T>((uint16_t)v), q.inv), qbyte(value_of<T>((uint16_t)(v >> 16)), q.inv));
+                    const uint32_t neg = (uint32_t)byte_lanes_negative(x);
+                    up[s][e] = (int)(x & ~neg);
+                    down[s][e] = (int)(x & neg);
+                }
+            if (half == 0) {
+                s_scale[wu * 32 + slot] = row ? q.sc : NAN;
+                s_last[wu * 32 + slot] = !row ? -1 : a.causal ? (int)tok + nk - nq : nk - 1;
+            }
+        }
+        // lane: column (a block); register r: slot 8 (r / 4) + 4 half + r % 4. A wave's own entries only: no barrier
+        float sc[16];
+        int least = nk - 1, most = -1;  // the last keys that its rows see
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int slot = wu * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+            sc[r] = s_scale[slot];
+            if (sc[r] == sc[r]) least = min(least, s_last[slot]), most = max(most, s_last[slot]);
+        }
+        least = min(least, __builtin_bit_cast(int, xor_lane<32>(__builtin_bit_cast(float, least))));
+        most = max(most, __builtin_bit_cast(int, xor_lane<32>(__builtin_bit_cast(float, most))));
+
+        if (pass) lds_barrier();  // the buffers' last readers are done
+        load(t0, 0);
+        const uint32_t rd = (uint32_t)((lane & 31) * 2 * D + ((half ^ (lane & 7)) << 4));
+        for (int t = t0; t < t1; t++) {
+            const int buf = (t - t0) & 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (t + 1 < t1) load(t + 1, buf ^ 1);
+            if (!live || (int64_t)32 * t * kKeyBlock > most) continue;
+            const unsigned char *sb = sc_smem + buf * TILE;
+            auto frag = [&](int s) { return *(const v4i *)(sb + (rd ^ (uint32_t)((s & 3) << 5)) + (s >> 2) * 128); };
+            v16i acc = {};
+            v4i f[4];
+#pragma unroll
+            for (int s = 0; s < (2 * NS < 4 ? 2 * NS : 4); s++) f[s] = frag(s);
+#pragma unroll
+            for (int s = 0; s < 2 * NS; s++) {
+                acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(s < NS ? up[s] : down[s - NS], f[s & 3], acc, 0, 0, 0);
+                if (s + 4 < 2 * NS) f[s & 3] = frag(s + 4);
+            }
+            const int n = 32 * t + (lane & 31);
+            float best[4];  // runs of 4 slots: register i of half h is slots 8 i + 4 h .. + 3
+            if ((int64_t)(32 * t + 31) * kKeyBlock <= least) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    best[i] = fmaxf(fmaxf(__fmul_rn((float)acc[4 * i], sc[4 * i]), __fmul_rn((float)acc[4 * i + 1], sc[4 * i + 1])),
+                                    fmaxf(__fmul_rn((float)acc[4 * i + 2], sc[4 * i + 2]), __fmul_rn((float)acc[4 * i + 3], sc[4 * i + 3])));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    best[i] = NAN;
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (n * kKeyBlock <= s_last[wu * 32 + 8 * i + 4 * half + e])
+                            best[i] = fmaxf(best[i], __fmul_rn((float)acc[4 * i + e], sc[4 * i + e]));
+                }
+            }
+            if (span > 1) {
+                float v = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+                v = fmaxf(v, xor_lane<32>(v));
+                if (half == 0 && v == v) atomicMax(s_best + blk * width + n - 32 * t0, order_key(v));
+                continue;
+            }
+            const float ks = n < nb ? a.kscale[((int64_t)b * a.NB + n) * a.KV + kvh] : 0.f;
+            auto put = [&](int i, float v) {
+                if (n < nb && (int64_t)(qb0 + blk + i) * a.q_block < nq)
+                    a.scores[(((int64_t)b * a.NQ + qb0 + blk + i) * a.KV + kvh) * a.NB + n] = __fmul_rn(v, ks);
+            };
+            if (a.group == 4) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) put(2 * i + half, best[i]);
+                continue;
+            }
+            float run[4];  // slots 8 i .. 8 i + 7
+#pragma unroll
+            for (int i = 0; i < 4; i++) run[i] = fmaxf(best[i], xor_lane<32>(best[i]));
+            if (half) continue;
+            if (a.group == 8) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) put(i, run[i]);
+            } else if (a.group == 16) {
+                put(0, fmaxf(run[0], run[1]));
+                put(1, fmaxf(run[2], run[3]));
+            } else {
+                put(0, fmaxf(fmaxf(run[0], run[1]), fmaxf(run[2], run[3])));
+            }
+        }
+    }
+    if (span == 1) return;
+    __syncthreads();
+    for (int i = tid; i < width * wg_blocks; i += 256) {
+        const int blk = i / width, n = 32 * t0 + i % width;
+        if (n >= nb || (int64_t)(qb0 + blk) * a.q_block >= nq) continue;
+        const float ks = a.kscale[((int64_t)b * a.NB + n) * a.KV + kvh];
+        a.scores[(((int64_t)b * a.NQ + qb0 + blk) * a.KV + kvh) * a.NB + n] = __fmul_rn(score_of(s_best[i]), ks);
+    }
+}
+
+__device__ inline uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    return v;
+}
+
+// The n_sel largest: the n_sel-th largest key by bisection of the bits in which the keys differ (counts by ballots
+// over keys held in registers), ended as soon as a count is n_sel; then everything above it and the first of its equals,
+// in block order. W waves a list, RPL keys a lane: key 64 (w RPL + j) + lane is register j of wave w.
 template <int W, int RPL>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_block_top(SelectArgs a, int64_t lists) {
     constexpr int WG = W > 4 ? W : 4;  // waves a workgroup
     __shared__ int s_n[W > 1 ? 2 : 1][W];
+    __shared__ uint32_t s_ends[2][W];
     const int lane = threadIdx.x & 63, w = W > 1 ? threadIdx.x >> 6 : 0;
     const int64_t id = (int64_t)blockIdx.x * (WG / W) + (W > 1 ? 0 : threadIdx.x >> 6);
     if (id >= lists) return;
@@ -263,15 +364,33 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_block_top(SelectArgs a
         return c;
     };
     int before;
-    uint32_t cut = 1;
-    int above = 0;  // keys > cut that are taken; equals fill the rest
-    if (total(count(1), before) > a.n_sel) {
-        cut = 0;
-        for (int bit = 31; bit >= 0; bit--) {
-            const uint32_t c = cut | (1u << bit);
-            if (total(count(c), before) >= a.n_sel) cut = c;
+    uint32_t cut = 1;  // keys > cut are taken; of its equals the first
+    int above;
+    const int forced = total(count(0xffffffffu), before);
+    if (total(count(1), before) > a.n_sel && forced < a.n_sel) {
+        // scores lie close together: the bits that all of them share need no counting
+        uint32_t hi = 1, lo = 0xfffffffeu;
+#pragma unroll
+        for (int j = 0; j < RPL; j++)
+            if (key[j] && key[j] != 0xffffffffu) hi = max(hi, key[j]), lo = min(lo, key[j]);
+        hi = wave_max(hi), lo = ~wave_max(~lo);
+        if constexpr (W > 1) {
+            if (lane == 0) s_ends[0][w] = hi, s_ends[1][w] = lo;
+            __syncthreads();
+            for (int i = 0; i < W; i++) hi = max(hi, s_ends[0][i]), lo = min(lo, s_ends[1][i]);
         }
-        above = cut == 0xffffffffu ? 0 : total(count(cut + 1), before);
+        const int bits = hi == lo ? 0 : 32 - __clz(hi ^ lo);
+        cut = bits < 32 ? hi >> bits << bits : 0;
+        for (int bit = bits - 1; bit >= 0; bit--) {
+            const uint32_t c = cut | (1u << bit);
+            const int n = total(count(c), before);
+            if (n >= a.n_sel) cut = c;
+            if (n == a.n_sel) break;
+        }
+        above = total(count(cut + 1), before);
+    } else if (forced >= a.n_sel) {
+        cut = 0xffffffffu;
+        above = 0;
     } else {
         above = total(count(2), before);
     }
@@ -285,8 +404,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_block_top(SelectArgs a
     }
     int eq_before, over_before;
     total(equal, eq_before);
-    const int n_over = total(over, over_before);
-    (void)n_over;
+    total(over, over_before);
     int eq = eq_before, at = over_before + min(eq_before, room);
     const uint64_t low = (1ull << lane) - 1;
 #pragma unroll
@@ -310,12 +428,22 @@ static int launch_bounds_of(hipStream_t st, const BoundsArgs &a, int B) {
 }
 template <class T, int D>
 static int launch_scores(hipStream_t st, const SelectArgs &a, int B) {
-    const int64_t tiles = ((int64_t)a.NQ * a.group + 31) / 32, grid = tiles * ((a.NB + 127) / 128);
+    const int span = (a.q_block * a.G + 31) / 32, wg_blocks = span > 4 ? 1 : span > 1 ? 4 / span : 128 / a.group;
+    const int64_t groups = ((int64_t)a.NQ + wg_blocks - 1) / wg_blocks, tiles = ((int64_t)a.NB + 31) / 32;
+    // shares of the blocks: two workgroups a CU, at most 128 tiles each (the maxima's LDS: 16 KB a query block)
+    int64_t shares = (2L * num_cus() + groups * a.KV * B - 1) / (groups * a.KV * B);
+    if (shares > tiles) shares = tiles;
+    if (shares < (tiles + 127) / 128) shares = (tiles + 127) / 128;
+    const int64_t grid = groups * shares * a.KV * B;
     if (grid > 0x7fffffff) {
         set_error("block_select: too many rows for a launch");
         return -1;
     }
-    hipLaunchKernelGGL((k_block_scores<T, D>), dim3((unsigned)grid, a.KV, B), dim3(256), 0, st, a);
+    const size_t lds = 128 * D + (span > 1 ? (size_t)((tiles + shares - 1) / shares) * 128 * wg_blocks : 0);
+    if (check_hip(hipFuncSetAttribute((const void *)k_block_scores<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
+                  "lds attribute"))
+        return -1;
+    hipLaunchKernelGGL((k_block_scores<T, D>), dim3((unsigned)grid), dim3(256), lds, st, a, (int)shares, (int)groups);
     return check_hip(hipGetLastError(), "block scores launch");
 }
 
@@ -401,7 +529,10 @@ extern "C" int e2mi_block_select(e2mi_stream stream, int dtype, const uint16_t *
         return -1;
     }
     const unsigned n = (unsigned)lists;
+    // a wave a list; four where the lists are too few to fill the device
+    const bool few = lists < 4L * num_cus();
     if (a.NB <= 512) hipLaunchKernelGGL((k_block_top<1, 8>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
+    else if (a.NB <= 2048 && few) hipLaunchKernelGGL((k_block_top<4, 8>), dim3(n), dim3(256), 0, st, a, lists);
     else if (a.NB <= 2048) hipLaunchKernelGGL((k_block_top<1, 32>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
     else if (a.NB <= 8192) hipLaunchKernelGGL((k_block_top<4, 32>), dim3(n), dim3(256), 0, st, a, lists);
     else hipLaunchKernelGGL((k_block_top<16, 32>), dim3(n), dim3(1024), 0, st, a, lists);
