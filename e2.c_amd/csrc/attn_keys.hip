@@ -229,7 +229,7 @@ __device__ inline f4v mma16(typename Half8<T>::type a, typename Half8<T>::type b
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 template <int D>
-constexpr size_t few_lds() { return 4 * 16 * (D + 4) * 4; }
+constexpr size_t few_lds() { return 4 * 16 * (D + 4) * 4 + 2 * 8 * D * 2; }
 
 template <class T, int D>
 __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) {
@@ -237,11 +237,17 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) 
     typedef T T4 __attribute__((ext_vector_type(4)));
     // V^T tiles held at once: at head_dim 512 half of them (all would spill), requested as the tile comes up
     constexpr int NQ = D / 32, NO = D / 16, PITCH = D + 4, NP = D == 512 ? 2 : 1, NV = NO / NP;
-    extern __shared__ __align__(16) float few_smem[];  // the waves' contexts [4][16][PITCH], then the list (kSelected)
+    extern __shared__ __align__(16) float few_smem[];  // the waves' contexts [4][16][PITCH]
     __shared__ float s_m[4][16], s_l[4][16];
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, g = lane >> 4;
-    int *list = (int *)(few_smem + 4 * 16 * PITCH);
+    // V^T of a range of under 8 keys, [dim][8] (the prefix's, the own), then the list (kSelected)
+    uint16_t *s_short = (uint16_t *)(few_smem + 4 * 16 * PITCH);
+    int *list = (int *)(s_short + 2 * 8 * D);
+    auto short_range = [&](const KeySet &src, int64_t col, int n, uint16_t *to) {
+        for (int i = tid; i < 8 * D; i += 256)
+            to[i] = (i & 7) < n ? src.vt[((int64_t)blockIdx.y * D + (i >> 3)) * src.ldv + col + (i & 7)] : 0;
+    };
     Walk k;
     if (!start_walk<16>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
                         &s_count, k))
@@ -260,49 +266,43 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) 
     for (int t = 0; t < NO; t++) o[t] = (f4v){};
     float mrun = -INFINITY, lrun = 0.f;
 
-    // tile t: where its keys lie; one without keys (the second half of a short last block) reads the first key and counts none
+    // tile t: where its keys lie; one without keys (the second half of a short last block) stands at the range's start
     auto place = [&](int t) {
         KeyTile kt = key_tile(a, k, list, t);
-        if (kt.n <= 0) kt.n = 0, kt.key0 = 0;
+        if (kt.n == 0) kt.key0 = 0;
         return kt;
     };
     V8 kf[2][NQ], vf[NV];
+    // The 8 keys of lane group x of a tile start at key 8 x, or 8 before the range's end where that comes sooner: no
+    // read leaves the range, so what lies past it (of any bits, or past the tensor) needs no clearing. Keys that come
+    // twice so, at most into the tile before, are masked where they are not 8 x or more.
+    auto first_of = [&](const KeyTile &kt, int x) { return max(min(8 * x, kt.n - 8), -kt.key0); };
     auto load_k = [&](const KeyTile &kt) {
         const KeySet &src = kt.pre ? a.pre : a.own;
-        const int64_t row = (kt.pre ? 0 : k.ks) + kt.key0;
+        const int key = (kt.pre ? 0 : k.ks) + kt.key0 + first_of(kt, c >> 2), end = (kt.pre ? a.pre.rows : k.ks + k.nk) - 1;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int key = max(0, min(8 * (c >> 2) + 4 * u + (c & 3), kt.n - 1));
-            const uint16_t *kp = src.k + (row + key) * src.ldk + (int64_t)k.kvh * D + 8 * g;
+            const uint16_t *kp = src.k + (int64_t)min(key + 4 * u + (c & 3), end) * src.ldk + (int64_t)k.kvh * D + 8 * g;
 #pragma unroll
             for (int s = 0; s < NQ; s++) kf[u][s] = *(const V8 *)(kp + 32 * s);
         }
     };
     auto load_v = [&](const KeyTile &kt, int piece) {
         const KeySet &src = kt.pre ? a.pre : a.own;
-        const uint16_t *vp = src.vt + ((int64_t)k.kvh * D + piece * (D / NP) + c) * src.ldv + (kt.pre ? 0 : k.ks) + kt.key0 + 8 * g;
-        if (kt.n == 32) {
+        const uint16_t *vp = src.vt + ((int64_t)k.kvh * D + piece * (D / NP) + c) * src.ldv + (kt.pre ? 0 : k.ks);
+        const int key = kt.key0 + first_of(kt, g);
+        if ((kt.pre ? a.pre.rows : k.nk) >= 8) {
 #pragma unroll
-            for (int t = 0; t < NV; t++) vf[t] = load8<T>(vp + (int64_t)t * 16 * src.ldv);
-        } else {
-            // values past the range are not read (they may lie past the tensor) and count as 0: a zero probability
-            // times an infinity would be a NaN
-            const int have = kt.n - 8 * g;
+            for (int t = 0; t < NV; t++) vf[t] = load8<T>(vp + key + (int64_t)t * 16 * src.ldv);
+        } else {  // a range of under 8 keys
+            const uint16_t *x = s_short + (kt.pre ? 0 : 8 * D) + 8 * (piece * (D / NP) + c);
 #pragma unroll
-            for (int t = 0; t < NV; t++) {
-                const uint16_t *x = vp + (int64_t)t * 16 * src.ldv;
-                V8 v = {};
-                if (have >= 8) {
-                    v = load8<T>(x);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 7; e++)
-                        if (e < have) v[e] = __builtin_bit_cast(T, x[e]);
-                }
-                vf[t] = v;
-            }
+            for (int t = 0; t < NV; t++) vf[t] = *(const V8 *)(x + 8 * 16 * t);
         }
     };
+    if (k.n_pre && a.pre.rows < 8) short_range(a.pre, 0, a.pre.rows, s_short);
+    if (k.nk > 0 && k.nk < 8) short_range(a.own, k.ks, k.nk, s_short + 8 * D);
+    __syncthreads();
     KeyTile now = {}, next = {};
     if (k.t0 + w < k.t1) {
         now = place(k.t0 + w);
@@ -326,9 +326,10 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) 
         for (int i = 0; i < 8; i++) tv[i] = st[i >> 2][i & 3];
         if (now.n < 32 || (!now.pre && a.causal)) {
             const int top = now.pre ? now.n - 1 : min(last - now.key0, now.n - 1);
+            const int first = first_of(now, g);
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (8 * g + i > top) tv[i] = -INFINITY;
+                if (first + i > top || first + i < 8 * g) tv[i] = -INFINITY;
         }
         float mloc = tv[0];
 #pragma unroll
