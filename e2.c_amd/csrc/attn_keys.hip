@@ -17,6 +17,8 @@
 // 16-byte chunks of 8 keys.
 #include <math.h>
 
+#include <type_traits>
+
 #include "attn_keys.h"
 
 namespace e2mi {
@@ -68,12 +70,11 @@ __device__ __forceinline__ float softmax_step(const float (&s)[16], float c, flo
     return alpha;
 }
 
-// 8 consecutive values at any 2-byte address (V^T's pitch may be odd): one 16-byte load, unaligned
+// 8 consecutive values at any 2-byte address: one 16-byte load, unaligned
 template <class T>
 __device__ inline typename Half8<T>::type load8(const uint16_t *p) {
-    typename Half8<T>::type v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
+    typedef typename Half8<T>::type __attribute__((aligned(2))) any8;
+    return *(const __attribute__((address_space(1))) any8 *)p;
 }
 
 __device__ inline int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
@@ -198,6 +199,18 @@ __device__ inline KeyTile key_tile(const KeysArgs &a, const Walk &w, const int *
     return k;
 }
 
+// The set a tile lies in, its fields selected one by one: by reference, the fields would be loaded again from the
+// arguments at every tile.
+__device__ inline KeySet set_of(const KeysArgs &a, bool pre) {
+    KeySet s;
+    s.k = pre ? a.pre.k : a.own.k;
+    s.vt = pre ? a.pre.vt : a.own.vt;
+    s.ldk = pre ? a.pre.ldk : a.own.ldk;
+    s.ldv = pre ? a.pre.ldv : a.own.ldv;
+    s.rows = pre ? a.pre.rows : a.own.rows;
+    return s;
+}
+
 // Leaves a row's share for k_keys_merge: no key: nothing but the maximum says so; a NaN sum (NaN rows) takes the
 // whole row with it.
 template <int D, int DW = D>
@@ -214,44 +227,92 @@ __device__ __forceinline__ void write_share(const KeysArgs &a, const f16v (&o)[D
             *(float4 *)(y + 32 * i + 8 * g) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
 }
 
-// Few rows: 16 a workgroup, whose four waves take every fourth key tile and are joined through LDS. Fragments go from
-// global memory to registers: a tile's K and V^T are read by one wave only, so LDS would hold them for nobody else.
-// Bound by HBM, hence by what is in flight: a wave's next K tile is requested when its logits are done, the next V^T
-// tile when its context is, 16 KB each at head_dim 256.
+// Few rows: 16 a workgroup, whose waves take every WV-th key tile of 32 and are joined through LDS. Bound by HBM, hence by
+// what is in flight: each wave has LDS for a K and a V^T tile of its own and requests the next K tile when its logits are
+// done, the next V^T tile when its context is (direct-to-LDS loads, no barrier: 128 KB in flight a CU at head_dim 256).
+// Fragments loaded from global memory straight into registers took four times as long: neighbouring lanes of an operand
+// hold different rows, so every 16 bytes were a request of their own.
 //
-// 16x16x32 MFMA: half the registers of the 32-row form for Q and the context, which is what lets the tiles in flight
-// fit. Logits of 32 keys are two products whose K rows are permuted (row 4 g + i of product u holds key 8 g + 4 u + i)
-// so that a lane ends with 8 consecutive keys of one row, the operand of the next product.
+// 16x16x32 MFMA. Logits of 32 keys are two products whose K rows are permuted (row 4 x + i of product u holds key
+// 8 x + 4 u + i), so that a lane ends with 8 consecutive keys of one row, the operand of the next product.
+// LDS: K row i (2 D bytes) holds key i, its 16-byte chunk x at position x ^ f(i); V^T row d (64 bytes) its chunk x at
+// x ^ ((d >> 2) & 3): 16 lanes of a read hit 16 bank groups.
 typedef float f4v __attribute__((ext_vector_type(4)));
 template <class T>
 __device__ inline f4v mma16(typename Half8<T>::type a, typename Half8<T>::type b, f4v c) {
-    if constexpr (sizeof(T) == 2 && __is_same(T, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    if constexpr (__is_same(T, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 template <int D>
-constexpr size_t few_lds() { return 4 * 16 * (D + 4) * 4 + 2 * 8 * D * 2; }
+struct FewTile {
+    static constexpr int WV = D == 512 ? 2 : 4;              // waves
+    static constexpr int kTile = 64 * D, kWave = 2 * kTile;  // bytes of a K (or V^T) tile; of a wave
+    static constexpr int PITCH = D + 4;                      // floats of a row when the waves are joined
+    static constexpr int kBytes = WV * kWave > WV * 16 * PITCH * 4 ? WV * kWave : WV * 16 * PITCH * 4;
+};
+// dma16 without a compiler memory clobber: the kernels order these loads with their reads by explicit waits
+__device__ inline void dma16_nc(v4u r, uint32_t lds, uint32_t voff, uint32_t soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff));
+}
+// x, not to be computed ahead for every load of a tile: that many scalars do not fit
+__device__ inline uint64_t here(uint64_t x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+__device__ inline uint32_t here(uint32_t x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
 
 template <class T, int D>
-__global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) {
+__global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
     typedef typename Half8<T>::type V8;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    // V^T tiles held at once: at head_dim 512 half of them (all would spill), requested as the tile comes up
-    constexpr int NQ = D / 32, NO = D / 16, PITCH = D + 4, NP = D == 512 ? 2 : 1, NV = NO / NP;
-    extern __shared__ __align__(16) float few_smem[];  // the waves' contexts [4][16][PITCH]
-    __shared__ float s_m[4][16], s_l[4][16];
+    using L = FewTile<D>;
+    constexpr int WV = L::WV, NQ = D / 32, NO = D / 16, PITCH = L::PITCH;
+    constexpr int RPI = 512 / D, LPR = D / 8, NL = D / 16;  // K rows a load fetches, lanes per K row, loads of a tile
+    extern __shared__ __align__(16) unsigned char few_smem[];  // the waves' tiles, then the list (kSelected)
+    __shared__ float s_m[WV][16], s_l[WV][16];
     __shared__ int s_count;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, g = lane >> 4;
-    // V^T of a range of under 8 keys, [dim][8] (the prefix's, the own), then the list (kSelected)
-    uint16_t *s_short = (uint16_t *)(few_smem + 4 * 16 * PITCH);
-    int *list = (int *)(s_short + 2 * 8 * D);
-    auto short_range = [&](const KeySet &src, int64_t col, int n, uint16_t *to) {
-        for (int i = tid; i < 8 * D; i += 256)
-            to[i] = (i & 7) < n ? src.vt[((int64_t)blockIdx.y * D + (i >> 3)) * src.ldv + col + (i & 7)] : 0;
-    };
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int *list = (int *)(few_smem + L::kBytes);
     Walk k;
     if (!start_walk<16>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
                         &s_count, k))
         return;
+    unsigned char *sk = few_smem + w * L::kWave, *sv = sk + L::kTile;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_void *)few_smem) + (uint32_t)(w * L::kWave);
+    const int lr = lane / LPR, lc = lane % LPR;
+    const int vchunk = (lane & 3) ^ ((lane >> 4) & 3);
+    auto f_of = [](int row) { return D == 64 ? ((row >> 1) & 1) | ((row >> 3) & 3) << 1 : (row & 3) | ((row >> 3) & 3) << 2; };
+    // descriptors start at a load's first row, so 32 bits hold every offset at any length of the cache
+    auto load_k = [&](const KeyTile &kt) {
+        const KeySet src = set_of(a, kt.pre);
+        const uint16_t *base = src.k + ((int64_t)(kt.pre ? 0 : k.ks) + kt.key0) * src.ldk + (int64_t)k.kvh * D;
+        const uint32_t ldB = (uint32_t)src.ldk * 2, bytes = kt.n ? (uint32_t)(kt.n - 1) * ldB + 2 * D : 0, ko = (uint32_t)lr * ldB;
+        const v4u rs = rsrc_words(base, bytes);  // a row past the range lies past its end: zeros
+        uint32_t at = 0;
+#pragma unroll
+        for (int j = 0; j < NL; j++, at = here(at + RPI * ldB))
+            dma16_nc(rs, lds0 + (uint32_t)(j * 1024), ko + (uint32_t)((lc ^ f_of(RPI * j + lr)) << 4), at);
+    };
+    auto load_v = [&](const KeyTile &kt) {
+        const KeySet src = set_of(a, kt.pre);
+        uint64_t base = (uint64_t)(src.vt + (int64_t)k.kvh * D * src.ldv + (kt.pre ? 0 : k.ks) + kt.key0);
+        const uint32_t ldB = (uint32_t)src.ldv * 2;
+        const uint32_t vo = 8 * vchunk < kt.n ? (uint32_t)(lane >> 2) * ldB + (uint32_t)vchunk * 16 : 0x80000000u;
+#pragma unroll
+        for (int j = 0; j < NL; j++, base = here(base + 16 * (uint64_t)ldB))
+            dma16_nc(rsrc_words((const void *)base, 0x7fffffffu), lds0 + (uint32_t)(L::kTile + j * 1024), vo, 0);
+    };
+    int t = k.t0 + w;
+    KeyTile now = {}, next = {};
+    if (t < k.t1) {
+        now = key_tile(a, k, list, t);
+        load_k(now);
+        load_v(now);
+    }
     int last;  // own keys this lane's row sees
     V8 qf[NQ];
     {
@@ -263,62 +324,28 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) 
     }
     f4v o[NO];
 #pragma unroll
-    for (int t = 0; t < NO; t++) o[t] = (f4v){};
+    for (int i = 0; i < NO; i++) o[i] = (f4v){};
     float mrun = -INFINITY, lrun = 0.f;
+    uint32_t krd[2];
+    const int fc = f_of(8 * (c >> 2) + (c & 3));  // the same for both products' rows
+#pragma unroll
+    for (int u = 0; u < 2; u++) krd[u] = (uint32_t)((8 * (c >> 2) + 4 * u + (c & 3)) * 2 * D);
+    const uint32_t vrd = (uint32_t)(c * 64 + ((g ^ ((c >> 2) & 3)) << 4));
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // everything so far; inside the loop the compiler must find nothing to wait for
 
-    // tile t: where its keys lie; one without keys (the second half of a short last block) stands at the range's start
-    auto place = [&](int t) {
-        KeyTile kt = key_tile(a, k, list, t);
-        if (kt.n == 0) kt.key0 = 0;
-        return kt;
-    };
-    V8 kf[2][NQ], vf[NV];
-    // The 8 keys of lane group x of a tile start at key 8 x, or 8 before the range's end where that comes sooner: no
-    // read leaves the range, so what lies past it (of any bits, or past the tensor) needs no clearing. Keys that come
-    // twice so, at most into the tile before, are masked where they are not 8 x or more.
-    auto first_of = [&](const KeyTile &kt, int x) { return max(min(8 * x, kt.n - 8), -kt.key0); };
-    auto load_k = [&](const KeyTile &kt) {
-        const KeySet &src = kt.pre ? a.pre : a.own;
-        const int key = (kt.pre ? 0 : k.ks) + kt.key0 + first_of(kt, c >> 2), end = (kt.pre ? a.pre.rows : k.ks + k.nk) - 1;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const uint16_t *kp = src.k + (int64_t)min(key + 4 * u + (c & 3), end) * src.ldk + (int64_t)k.kvh * D + 8 * g;
-#pragma unroll
-            for (int s = 0; s < NQ; s++) kf[u][s] = *(const V8 *)(kp + 32 * s);
-        }
-    };
-    auto load_v = [&](const KeyTile &kt, int piece) {
-        const KeySet &src = kt.pre ? a.pre : a.own;
-        const uint16_t *vp = src.vt + ((int64_t)k.kvh * D + piece * (D / NP) + c) * src.ldv + (kt.pre ? 0 : k.ks);
-        const int key = kt.key0 + first_of(kt, g);
-        if ((kt.pre ? a.pre.rows : k.nk) >= 8) {
-#pragma unroll
-            for (int t = 0; t < NV; t++) vf[t] = load8<T>(vp + key + (int64_t)t * 16 * src.ldv);
-        } else {  // a range of under 8 keys
-            const uint16_t *x = s_short + (kt.pre ? 0 : 8 * D) + 8 * (piece * (D / NP) + c);
-#pragma unroll
-            for (int t = 0; t < NV; t++) vf[t] = *(const V8 *)(x + 8 * 16 * t);
-        }
-    };
-    if (k.n_pre && a.pre.rows < 8) short_range(a.pre, 0, a.pre.rows, s_short);
-    if (k.nk > 0 && k.nk < 8) short_range(a.own, k.ks, k.nk, s_short + 8 * D);
-    __syncthreads();
-    KeyTile now = {}, next = {};
-    if (k.t0 + w < k.t1) {
-        now = place(k.t0 + w);
-        load_k(now);
-        if (NP == 1) load_v(now, 0);
-    }
-    for (int t = k.t0 + w; t < k.t1; t += 4, now = next) {
-        const bool more = t + 4 < k.t1;
-        if (NP > 1) load_v(now, 0);
+    for (; t < k.t1; t += WV, now = next) {
+        const bool more = t + WV < k.t1;
+        // the tile's K has landed (V^T was requested after it)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
         f4v st[2] = {};
 #pragma unroll
         for (int s = 0; s < NQ; s++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) st[u] = mma16<T>(kf[u][s], qf[s], st[u]);
+            for (int u = 0; u < 2; u++)
+                st[u] = mma16<T>(*(const V8 *)(sk + krd[u] + (((4 * s + g) ^ fc) << 4)), qf[s], st[u]);
         if (more) {
-            next = place(t + 4);
+            next = key_tile(a, k, list, t + WV);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its reads are done
             load_k(next);
         }
         float tv[8];
@@ -326,10 +353,9 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) 
         for (int i = 0; i < 8; i++) tv[i] = st[i >> 2][i & 3];
         if (now.n < 32 || (!now.pre && a.causal)) {
             const int top = now.pre ? now.n - 1 : min(last - now.key0, now.n - 1);
-            const int first = first_of(now, g);
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (first + i > top || first + i < 8 * g) tv[i] = -INFINITY;
+                if (8 * g + i > top) tv[i] = -INFINITY;
         }
         float mloc = tv[0];
 #pragma unroll
@@ -337,9 +363,10 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) 
         mloc = fmaxf(mloc, xor_lane<16>(mloc));
         mloc = fmaxf(mloc, xor_lane<32>(mloc));
         const float mc = mloc * a.c2;
-        if (mc > mrun + kTau) {
-            const float alpha = __builtin_amdgcn_exp2f(mrun - mc);
-            mrun = mc;
+        const bool moved = mc > mrun + kTau;
+        if (__any(moved)) {
+            const float alpha = moved ? __builtin_amdgcn_exp2f(mrun - mc) : 1.f;
+            mrun = moved ? mc : mrun;
             lrun *= alpha;
 #pragma unroll
             for (int i = 0; i < NO; i++) o[i] *= alpha;
@@ -352,37 +379,49 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void k_keys_few(KeysArgs a) 
             lrun += p;
             pb[i] = (T)p;
         }
+        // the tile's V^T has landed (the next K was requested after it)
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (now.n & 7) {  // values past the range in its last chunk (of any bits) become 0
+            const int have = now.n & 7;
+            for (int d = lane; d < D; d += 64) {
+                uint32_t *x = (uint32_t *)(sv + d * 64 + (((now.n >> 3) ^ ((d >> 2) & 3)) << 4));
 #pragma unroll
-        for (int i = 0; i < NV; i++) o[i] = mma16<T>(vf[i], pb, o[i]);
-        if constexpr (NP > 1) {
-            load_v(now, 1);
+                for (int e = 0; e < 4; e++) x[e] &= have >= 2 * e + 2 ? 0xffffffffu : have == 2 * e + 1 ? 0xffffu : 0u;
+            }
+        }
 #pragma unroll
-            for (int i = 0; i < NV; i++) o[NV + i] = mma16<T>(vf[i], pb, o[NV + i]);
-        } else if (more) {
-            load_v(next, 0);
+        for (int i = 0; i < NO; i++) o[i] = mma16<T>(*(const V8 *)(sv + vrd + i * 1024), pb, o[i]);
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load_v(next);
         }
     }
 
-    // join the four waves: contexts as they are, with their maxima and sums; a quad of dims a thread
+    // join the waves: contexts as they are, with their maxima and sums; a quad of dims a thread
     float lsum = lrun + xor_lane<16>(lrun);
     lsum += xor_lane<32>(lsum);
     if (g == 0) s_m[w][c] = mrun, s_l[w][c] = lsum;
+    __syncthreads();  // the tiles are read
+    float *ctx = (float *)few_smem;
     {
-        float *y = few_smem + (w * 16 + c) * PITCH + 4 * g;
+        float *y = ctx + (w * 16 + c) * PITCH + 4 * g;
 #pragma unroll
         for (int i = 0; i < NO; i++) *(f4v *)(y + 16 * i) = o[i];
     }
     __syncthreads();
+#pragma unroll 1
+    for (int at = tid; at < 4 * D; at += 64 * WV) {
+        const int row = at / (D / 4), d = at % (D / 4) * 4, r = k.r0 + row;
+        float mall = s_m[0][row];
 #pragma unroll
-    for (int i = 0; i < D / 64; i++) {
-        const int at = tid + 256 * i, row = at / (D / 4), d = at % (D / 4) * 4, r = k.r0 + row;
-        const float mall = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+        for (int x = 1; x < WV; x++) mall = fmaxf(mall, s_m[x][row]);
         f4v v = {};
         float sum = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
+        for (int x = 0; x < WV; x++) {
             const float mx = s_m[x][row], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mall);
-            v += *(const f4v *)(few_smem + (x * 16 + row) * PITCH + d) * f;
+            v += *(const f4v *)(ctx + (x * 16 + row) * PITCH + d) * f;
             sum += s_l[x][row] * f;
         }
         if (sum != sum) v = (f4v)NAN;
@@ -432,9 +471,6 @@ struct WideTile {
     static constexpr int kX = kV + 2 * kTile;       // the exchange: 4 KB a wave
     static constexpr int bytes(int nw) { return kX + (DS > 1 ? nw * DS * 4096 : 0); }
 };
-__device__ inline void dma16_nc(v4u r, uint32_t lds, uint32_t voff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r));
-}
 // K and V^T fragments are read this many MFMAs ahead of their use
 constexpr int kAhead = 3;
 
@@ -494,7 +530,7 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
         uint32_t ko, vo;           // lane offsets
     };
     auto fetch_of = [&](const KeyTile &kt) {
-        const KeySet &src = kt.pre ? a.pre : a.own;
+        const KeySet src = set_of(a, kt.pre);
         const int64_t row = (kt.pre ? 0 : k.ks) + kt.key0;
         Fetch f;
         f.k = src.k + row * src.ldk + (int64_t)k.kvh * D;
@@ -509,14 +545,13 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
         const int x = NLW * wu + j, i = RPI * x;
         if (NL % WV && x >= NL) return;
         // a row past the range reads as zero: the lane offset lies past the descriptor's end
-        const uint32_t key = (uint32_t)swap23(i) * f.ldk;
-        const v4u rs = rsrc_words((const char *)f.k + key, key < f.bytes ? f.bytes - key : 0);
-        dma16_nc(rs, lds0 + (uint32_t)(buf * L::kTile + i * (2 * D)), f.ko + (uint32_t)((lc ^ ((i + lr) & 7)) << 4));
+        dma16_nc(rsrc_words(f.k, f.bytes), lds0 + (uint32_t)(buf * L::kTile + i * (2 * D)),
+                 f.ko + (uint32_t)((lc ^ ((i + lr) & 7)) << 4), here((uint32_t)swap23(i) * f.ldk));
     };
     auto load_v = [&](const Fetch &f, int buf, int j) {
         if (NL % WV && NLW * wu + j >= NL) return;
-        const v4u rs = rsrc_words((const char *)f.v + (uint64_t)(16 * j) * f.ldv, 0x7fffffffu);
-        dma16_nc(rs, lds0 + (uint32_t)(L::kV + buf * L::kTile + (NLW * wu + j) * 1024), f.vo);
+        const v4u rs = rsrc_words((const void *)here((uint64_t)f.v + (uint64_t)(16 * j) * f.ldv), 0x7fffffffu);
+        dma16_nc(rs, lds0 + (uint32_t)(L::kV + buf * L::kTile + (NLW * wu + j) * 1024), f.vo, 0);
     };
 
     const int kkey = lane & 31;
@@ -639,7 +674,7 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
     write_row<T, D, DW>(a, o, m, h, l >> 5, dim0);
 }
 
-// V^T rows of any pitch and address, copied to a pitch that 16-byte loads take (k_keys_wide).
+// V^T rows of any pitch and address, copied to a pitch that 16-byte loads take.
 __global__ __launch_bounds__(256) void k_pad_rows(uint16_t *y, int64_t ldy, const uint16_t *x, int64_t ldx, int n) {
     const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
     const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
@@ -647,11 +682,9 @@ __global__ __launch_bounds__(256) void k_pad_rows(uint16_t *y, int64_t ldy, cons
     const uint16_t *from = x + row * ldx + c;
     uint16_t *to = y + row * ldy + c;
     if (c + 8 <= n) {
-        uint4 v;
-        __builtin_memcpy(&v, from, 16);
-        *(uint4 *)to = v;
+        *(h8 *)to = load8<_Float16>(from);
     } else {
-        for (int e = 0; c + e < n; e++) to[e] = from[e];
+        for (int e = 0; e < 8; e++) to[e] = c + e < n ? from[e] : 0;
     }
 }
 
@@ -736,7 +769,7 @@ struct RowsPlan {
 struct KeysPlan {
     bool apart = false;  // the prefix by rows of all sequences, their own keys by sequence
     RowsPlan pre, rows;  // pre: the prefix's launch (apart)
-    size_t pad_pre = 0, pad_own = 0;  // bytes of V^T copies (k_keys_wide over odd pitches)
+    size_t pad_pre = 0, pad_own = 0;  // bytes of V^T copies (pitches off 16 bytes)
     int all() const { return (apart ? pre.parts : 0) + rows.parts; }
 };
 
@@ -751,43 +784,39 @@ static int key_shares(int64_t groups, int64_t tiles, int least, int most) {
 }
 
 // groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles
-static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int most, bool wide) {
+static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int most) {
     RowsPlan p;
-    p.nw = !wide || rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
+    p.nw = rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
     const int R = p.nw ? 32 * p.nw : 16;
     p.tiles = (rows + R - 1) / R;
     p.parts = key_shares(p.tiles * count, tiles, 8, most);
     return p;
 }
 
-static bool odd_pitch(int64_t ld, int rows) { return rows > 0 && ld % 8; }
-// k_keys_wide's loads are 16 bytes and keep 32-bit offsets within a tile of keys and 16 rows of V^T
-static bool wide_takes(const KeySet &s) {
-    return !s.rows || (s.ldk < (1 << 24) && s.ldv < (1 << 25));
-}
+// V^T of a pitch that 16-byte loads do not take is copied to one that they do
+static bool needs_copy(const KeySet &s) { return s.rows > 0 && s.ldv % 8; }
 static size_t pad_bytes(int rows, int KV, int D) { return ((size_t)rows + 7) / 8 * 16 * KV * D; }
 
 static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B, int max_q, int max_k, int H, int KV, int D) {
     KeysPlan p;
     const int G = H / KV, P = pre.rows;
-    const bool wide = wide_takes(own) && wide_takes(pre);
     const int64_t own_tiles = own.rows ? ((int64_t)max_k + 31) / 32 : 0, pre_tiles = ((int64_t)P + 31) / 32;
     const int64_t rows = (int64_t)max_q * G;
     // sequences of less than a tile share the prefix's tiles
     p.apart = B > 1 && P > 0 && rows < 32;
-    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, kMaxKeyParts / 2, wide);
-    p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), p.apart ? kMaxKeyParts / 2 : kMaxKeyParts, wide);
-    if (odd_pitch(pre.ldv, P) && (p.apart ? p.pre.nw : p.rows.nw)) p.pad_pre = pad_bytes(P, KV, D);
-    if (odd_pitch(own.ldv, own.rows) && p.rows.nw) p.pad_own = pad_bytes(own.rows, KV, D);
+    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, kMaxKeyParts / 2);
+    p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), p.apart ? kMaxKeyParts / 2 : kMaxKeyParts);
+    if (needs_copy(pre)) p.pad_pre = pad_bytes(P, KV, D);
+    if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
 }
 
 static KeysPlan plan_blocks(const KeySet &own, int B, int max_q, int H, int KV, int D, int q_block, int n_sel) {
     KeysPlan p;
     const int64_t NQ = ((int64_t)max_q + q_block - 1) / q_block;
-    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, kMaxKeyParts, wide_takes(own));
+    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, kMaxKeyParts);
     p.rows.tiles *= NQ;
-    if (odd_pitch(own.ldv, own.rows) && p.rows.nw) p.pad_own = pad_bytes(own.rows, KV, D);
+    if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
 }
 
@@ -817,15 +846,15 @@ static int launch_rows(hipStream_t st, KeysArgs a, const RowsPlan &p, int B) {
     if (p.nw == 2) return launch_wide<T, D, 2>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 3) return launch_wide<T, D, 3>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 4) return launch_wide<T, D, 4>(st, a, p.tiles, grid * a.KV * B);
-    const size_t lds = few_lds<D>() + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
+    const size_t lds = FewTile<D>::kBytes + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
     if (check_hip(hipFuncSetAttribute((const void *)k_keys_few<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
                   "lds attribute"))
         return -1;
-    hipLaunchKernelGGL((k_keys_few<T, D>), dim3((unsigned)grid, a.KV, B), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((k_keys_few<T, D>), dim3((unsigned)grid, a.KV, B), dim3(64 * FewTile<D>::WV), lds, st, a);
     return check_hip(hipGetLastError(), "attention launch");
 }
 
-// a copy of a set's V^T in rows of 16-byte multiples at `to`
+// a copy of a set's V^T in rows of 16-byte multiples at `to` (columns past its rows: zeros)
 static int pad_values(hipStream_t st, KeySet &s, int KV, int D, uint16_t *to) {
     const int64_t ld = ((int64_t)s.rows + 7) / 8 * 8;
     hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)((ld + 2047) / 2048), D, KV), dim3(256), 0, st, to, ld, s.vt, s.ldv, s.rows);
@@ -880,9 +909,9 @@ static bool sizes_fit(int Mq, int B, int max_q, int max_k, int H, int KV, int D)
 
 static int check_keys(const char *who, const char *what, const KeySet &s, int KV, int D) {
     if (s.rows < 0 || (s.rows && (!s.k || !s.vt || !aligned16(s.k) || (uintptr_t)s.vt % (s.ldv % 8 ? 2 : 16) || s.ldk < (int64_t)KV * D ||
-                                  s.ldk % 8 || s.ldv < s.rows || s.ldk > (1LL << 28) || s.ldv > (1LL << 31)))) {
-        set_error("%s: %s need 16-byte aligned k rows of a pitch >= KV * D in multiples of 8 and transposed v of a pitch >= "
-                  "rows, 16-byte aligned where that is a multiple of 8 (rows=%d ldk=%lld ldv=%lld)", who, what, s.rows, (long long)s.ldk, (long long)s.ldv);
+                                  s.ldk % 8 || s.ldv < s.rows || s.ldk >= (1 << 24) || s.ldv >= (1 << 26)))) {
+        set_error("%s: %s need 16-byte aligned k rows of a pitch >= KV * D in multiples of 8, below 2^24, and transposed v of a "
+                  "pitch >= rows, below 2^26, 16-byte aligned where that is a multiple of 8 (rows=%d ldk=%lld ldv=%lld)", who, what, s.rows, (long long)s.ldk, (long long)s.ldv);
         return -1;
     }
     return 0;

@@ -17,7 +17,7 @@ NOTHING = dict(B=0)  # what is checked, and then has nothing to do
 ROWS = [dict(dtype=2), dict(dtype=-1), dict(Mq=-1), dict(B=-1), dict(B=65536), dict(max_q=-1), dict(max_k=-1), dict(H=0), dict(KV=0),
         dict(KV=2), dict(D=96), dict(D=0), dict(q=None), dict(q=X + 8), dict(ldq=767), dict(ldq=772), dict(ldq=1 << 40), dict(qs=None),
         dict(ql=None), dict(kl=None)]
-KEYS = [dict(k=None), dict(k=2 * X + 2), dict(ldk=255), dict(ldk=260), dict(vt=None), dict(vt=3 * X + 1), dict(vt=3 * X + 2), dict(ldv=63), dict(Mk=-1),
+KEYS = [dict(k=None), dict(k=2 * X + 2), dict(ldk=255), dict(ldk=260), dict(vt=None), dict(vt=3 * X + 1), dict(vt=3 * X + 2), dict(ldv=63), dict(ldv=1 << 26), dict(ldk=1 << 24), dict(Mk=-1),
         dict(ks=None)]
 OUT = [dict(ctx=None), dict(ctx=10 * X + 4), dict(ldc=760), dict(ldc=770), dict(cq=X), dict(cs=X), dict(ctx=None, cq=X), dict(cq=X + 4, cs=X),
        dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan"))]
