@@ -62,4 +62,18 @@ __device__ inline bool key_range(const int32_t *start, const int32_t *len, int b
     return true;
 }
 
+// Allows a kernel `bytes` of dynamic LDS, once a device for its largest need so far (`allowed`: a static of the caller's,
+// one for each kernel; two threads at once ask twice).
+struct LdsAllowed {
+    int bytes[64] = {};
+};
+inline int allow_lds(const void *kernel, int bytes, LdsAllowed &allowed) {
+    int dev = 0;
+    if (check_hip(hipGetDevice(&dev), "device")) return -1;
+    if (dev < 64 && allowed.bytes[dev] >= bytes) return 0;
+    if (check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "lds attribute")) return -1;
+    if (dev < 64) allowed.bytes[dev] = bytes;
+    return 0;
+}
+
 }  // namespace e2mi

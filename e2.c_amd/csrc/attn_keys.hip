@@ -828,9 +828,8 @@ static size_t workspace_of(const KeysPlan &p, int Mq, int H, int D) { return par
 template <class T, int D, int NW>
 static int launch_wide(hipStream_t st, const KeysArgs &a, int64_t tiles, int64_t grid) {
     const size_t lds = WideTile<D>::bytes(NW) + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
-    if (check_hip(hipFuncSetAttribute((const void *)k_keys_wide<T, D, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
-                  "lds attribute"))
-        return -1;
+    static LdsAllowed allowed;
+    if (allow_lds((const void *)k_keys_wide<T, D, NW>, (int)lds, allowed)) return -1;
     hipLaunchKernelGGL((k_keys_wide<T, D, NW>), dim3((unsigned)grid), dim3(64 * NW * WideTile<D>::DS), lds, st, a, (int)tiles);
     return check_hip(hipGetLastError(), "attention launch");
 }
@@ -847,9 +846,8 @@ static int launch_rows(hipStream_t st, KeysArgs a, const RowsPlan &p, int B) {
     if (p.nw == 3) return launch_wide<T, D, 3>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 4) return launch_wide<T, D, 4>(st, a, p.tiles, grid * a.KV * B);
     const size_t lds = FewTile<D>::kBytes + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
-    if (check_hip(hipFuncSetAttribute((const void *)k_keys_few<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
-                  "lds attribute"))
-        return -1;
+    static LdsAllowed allowed;
+    if (allow_lds((const void *)k_keys_few<T, D>, (int)lds, allowed)) return -1;
     hipLaunchKernelGGL((k_keys_few<T, D>), dim3((unsigned)grid, a.KV, B), dim3(64 * FewTile<D>::WV), lds, st, a);
     return check_hip(hipGetLastError(), "attention launch");
 }

@@ -170,6 +170,7 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
                   (uint32_t)(r + lr) * ldb + (uint32_t)((lc ^ ((r + lr) & 7)) << 4), 0);
         }
     };
+    load(t0, 0);  // in flight while the rows are quantized
     const int passes = span > 4 ? (span + 3) / 4 : 1;
     for (int pass = 0; pass < passes; pass++) {
         // this wave's slot: query block `blk` (of the workgroup; span 1: its first), rows from r0 of it
@@ -225,8 +226,10 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
         least = min(least, __builtin_bit_cast(int, xor_lane<32>(__builtin_bit_cast(float, least))));
         most = max(most, __builtin_bit_cast(int, xor_lane<32>(__builtin_bit_cast(float, most))));
 
-        if (pass) lds_barrier();  // the buffers' last readers are done
-        load(t0, 0);
+        if (pass) {
+            lds_barrier();  // the buffers' last readers are done
+            load(t0, 0);
+        }
         const uint32_t rd = (uint32_t)((lane & 31) * 2 * D + ((half ^ (lane & 7)) << 4));
         for (int t = t0; t < t1; t++) {
             const int buf = (t - t0) & 1;
@@ -440,9 +443,8 @@ static int launch_scores(hipStream_t st, const SelectArgs &a, int B) {
         return -1;
     }
     const size_t lds = 128 * D + (span > 1 ? (size_t)((tiles + shares - 1) / shares) * 128 * wg_blocks : 0);
-    if (check_hip(hipFuncSetAttribute((const void *)k_block_scores<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
-                  "lds attribute"))
-        return -1;
+    static LdsAllowed allowed;
+    if (allow_lds((const void *)k_block_scores<T, D>, (int)lds, allowed)) return -1;
     hipLaunchKernelGGL((k_block_scores<T, D>), dim3((unsigned)grid), dim3(256), lds, st, a, (int)shares, (int)groups);
     return check_hip(hipGetLastError(), "block scores launch");
 }
@@ -529,9 +531,10 @@ extern "C" int e2mi_block_select(e2mi_stream stream, int dtype, const uint16_t *
         return -1;
     }
     const unsigned n = (unsigned)lists;
-    // a wave a list; four where the lists are too few to fill the device
+    // a wave a list, keys in registers; past 1024 blocks four where the lists are too few to fill the device
     const bool few = lists < 4L * num_cus();
     if (a.NB <= 512) hipLaunchKernelGGL((k_block_top<1, 8>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
+    else if (a.NB <= 1024) hipLaunchKernelGGL((k_block_top<1, 16>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
     else if (a.NB <= 2048 && few) hipLaunchKernelGGL((k_block_top<4, 8>), dim3(n), dim3(256), 0, st, a, lists);
     else if (a.NB <= 2048) hipLaunchKernelGGL((k_block_top<1, 32>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
     else if (a.NB <= 8192) hipLaunchKernelGGL((k_block_top<4, 32>), dim3(n), dim3(256), 0, st, a, lists);

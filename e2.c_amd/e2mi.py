@@ -8,6 +8,7 @@ streams), passed to the library as raw pointers. There is no fallback: if the li
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -756,31 +757,53 @@ def gather_ids(ids, rowmap, stream=None):
 
 
 # ---- long contexts: rotary positions, a shared prefix, selected key blocks
-_DTYPES = {}
-
-
-def _dtype(*tensors):
-    """The library's code of the tensors' one type; they lie on the current device, rows contiguous."""
+# Single tokens are calls of a few microseconds: each operand is looked at once, and sizes that follow from sizes are
+# kept (functools.lru_cache).
+@functools.lru_cache(maxsize=None)
+def _dtype_codes():
     import torch
-    if not _DTYPES:
-        _DTYPES.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
-    dev, kind = torch._C._cuda_getDevice(), tensors[0].dtype
-    for t in tensors:
-        if t.dtype != kind or kind not in _DTYPES:
-            raise E2MIError(f"needs tensors of one type (f16, bf16 or f32), got {t.dtype} with {kind}")
-        if t.device.type != "cuda" or t.get_device() != dev:
-            raise E2MIError(f"needs tensors on the current device {dev}, got one on {t.device}")
-        if t.stride(-1) != 1 and t.shape[-1] != 1:
-            raise E2MIError("needs rows of contiguous values")
-    return _DTYPES[kind]
+    return {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def _i32(dev, n, **named):
-    """Checks of device index arrays: int32, contiguous, on the tensors' device, n entries."""
+def _kind(name, t):
+    """The library's code of a tensor's type, and its device, which has to be the current one."""
     import torch
-    for name, t in named.items():
-        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous() or t.numel() < n:
-            raise E2MIError(f"{name} needs at least {n} contiguous int32 values on {dev}")
+    kind, dev = _dtype_codes().get(t.dtype), t.get_device()
+    if kind is None:
+        raise E2MIError(f"{name}: needs f16, bf16 or f32 rows, got {t.dtype}")
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise E2MIError(f"{name}: needs tensors on the current device, got one on {t.device}")
+    return kind, dev
+
+
+def _rows(name, t, rows, width, dtype, dev):
+    """Address and pitch of a tensor [rows, width] with contiguous rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != rows or shape[1] != width:
+        raise E2MIError(f"{name}: needs rows [{rows}, {width}], got {tuple(shape)}")
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise E2MIError(f"{name}: needs {dtype} tensors on device {dev}, got {t.dtype} on {t.device}")
+    if stride[1] != 1 and width > 1:
+        raise E2MIError(f"{name}: needs rows of contiguous values")
+    return t.data_ptr(), stride[0] if rows > 1 else max(stride[0], width)
+
+
+def _indices(name, t, n, dev):
+    """Address of a contiguous int32 device array of at least n entries."""
+    import torch
+    if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous() or t.numel() < n:
+        raise E2MIError(f"{name}: needs contiguous int32 arrays of at least {n} values on device {dev}")
+    return t.data_ptr()
+
+
+def _new(stream, make, *a, **kw):
+    """A new tensor for work on `stream` (None: the current one): allocated there, so that its memory is not
+    handed to other work before that stream is done with it."""
+    if stream is None:
+        return make(*a, **kw)
+    import torch
+    with torch.cuda.stream(stream):
+        return make(*a, **kw)
 
 
 def rope_freqs(rot_dim, theta=10000.0, scaling="plain", factor=1.0, trained_len=0, turns=(1.0, 32.0)):
@@ -799,83 +822,85 @@ def rope(q, k, pos, freqs, H, KV, layout="half", magnitude=1.0, inverse=False, q
     freqs float64 [rot_dim / 2] on the device. Returns (q_out, k_out), new tensors unless given (in
     place: q_out=q)."""
     import torch
-    given = [t for t in (q, k, q_out, k_out) if t is not None]
-    if q is None and k is None:
+    x, heads = (q, H) if q is not None else (k, KV)
+    if x is None:
         raise E2MIError("rope: needs q or k")
-    kind = _dtype(*given)
-    x = q if q is not None else k
-    M, dev = x.shape[0], x.device
-    D = q.shape[1] // H if q is not None else k.shape[1] // KV
-    for t, n in ((q, H), (q_out, H), (k, KV), (k_out, KV)):
-        if t is not None and (t.dim() != 2 or t.shape[0] != M or t.shape[1] != n * D):
-            raise E2MIError(f"rope: needs rows [{M}, {n} * {D}], got {tuple(t.shape)}")
-    _i32(dev, M, pos=pos)
-    if freqs.dtype != torch.float64 or freqs.device != dev or not freqs.is_contiguous():
-        raise E2MIError(f"rope: needs contiguous float64 frequencies on {dev}")
-    if q is not None and q_out is None:
-        q_out = _on(stream, lambda: torch.empty((M, H * D), dtype=q.dtype, device=dev))
-    if k is not None and k_out is None:
-        k_out = _on(stream, lambda: torch.empty((M, KV * D), dtype=k.dtype, device=dev))
-    ld = lambda t: 0 if t is None else t.stride(0) if M > 1 else max(t.stride(0), t.shape[1])  # noqa: E731
-    check(load().e2mi_rope(_stream(stream), kind, {"half": 0, "interleaved": 1}[layout], int(inverse), _p(q), ld(q),
-                           _p(q_out), ld(q_out), 0 if q is None else H, _p(k), ld(k), _p(k_out), ld(k_out),
-                           0 if k is None else KV, M, D, _p(pos), _p(freqs), 2 * freqs.numel(), magnitude), "rope")
+    kind, dev = _kind("rope", x)
+    dtype, (M, width) = x.dtype, x.shape
+    if heads <= 0 or width % heads:
+        raise E2MIError(f"rope: {width} values are not {heads} heads")
+    D = width // heads
+    pq = pk = po = pt = None
+    lq = lk = lo = lt = nq = nk = 0
+    if q is not None:
+        pq, lq = _rows("rope", q, M, width, dtype, dev)
+        nq = H
+        if q_out is None:
+            q_out = _new(stream, q.new_empty, (M, width))
+        po, lo = _rows("rope", q_out, M, width, dtype, dev)
+    if k is not None:
+        pk, lk = _rows("rope", k, M, KV * D, dtype, dev)
+        nk = KV
+        if k_out is None:
+            k_out = _new(stream, k.new_empty, (M, KV * D))
+        pt, lt = _rows("rope", k_out, M, KV * D, dtype, dev)
+    if freqs.dtype is not torch.float64 or freqs.get_device() != dev or not freqs.is_contiguous():
+        raise E2MIError(f"rope: needs contiguous float64 frequencies on device {dev}")
+    check(load().e2mi_rope(_stream(stream), kind, _LAYOUTS[layout], 1 if inverse else 0, pq, lq, po, lo, nq, pk, lk, pt, lt, nk, M,
+                           D, _indices("rope", pos, M, dev), freqs.data_ptr(), 2 * freqs.numel(), magnitude), "rope")
     return q_out, k_out
 
 
-def _on(stream, make):
-    """A new tensor for work on `stream` (None: the current one): allocated there, so that its memory is not
-    handed to other work before that stream is done with it."""
-    if stream is None:
-        return make()
-    import torch
-    with torch.cuda.stream(stream):
-        return make()
+_LAYOUTS = {"half": 0, "interleaved": 1}
+_NO_KEYS = (None, 0, None, 0, 0)
 
 
-def _keys_of(name, k, vt, KV, D):
-    """(k, its pitch, vt, its pitch, rows) of keys k [rows, KV * D] and vt [KV, D, columns >= rows]."""
+def _keys(name, k, vt, KV, D, dtype, dev):
+    """(address of k, its pitch, of vt, its pitch, rows) of keys k [rows, KV * D] and vt [KV, D, columns >= rows]."""
     if k is None or k.shape[0] == 0:
-        return None, 0, None, 0, 0
-    if k.dim() != 2 or k.shape[1] != KV * D or vt.dim() != 3 or vt.shape[0] != KV or vt.shape[1] != D or vt.shape[2] < k.shape[0]:
-        raise E2MIError(f"{name}: needs k [rows, {KV * D}] and vt [{KV}, {D}, >= rows], got {tuple(k.shape)} and {tuple(vt.shape)}")
-    if vt.stride(0) != D * vt.stride(1):
-        raise E2MIError(f"{name}: needs vt's kv heads one after the other (a head pitch of D rows)")
-    return _p(k), k.stride(0) if k.shape[0] > 1 else max(k.stride(0), KV * D), _p(vt), vt.stride(1), k.shape[0]
+        return _NO_KEYS
+    rows = k.shape[0]
+    address, pitch = _rows(name, k, rows, KV * D, dtype, dev)
+    shape, stride = vt.shape, vt.stride()
+    if len(shape) != 3 or shape[0] != KV or shape[1] != D or shape[2] < rows:
+        raise E2MIError(f"{name}: needs vt [{KV}, {D}, >= {rows}], got {tuple(shape)}")
+    if vt.dtype is not dtype or vt.get_device() != dev or stride[2] != 1 or (KV > 1 and stride[0] != D * stride[1]):
+        raise E2MIError(f"{name}: needs {dtype} vt on device {dev}, columns contiguous, its kv heads one after the other")
+    return address, pitch, vt.data_ptr(), stride[1], rows
 
 
-def _contexts(name, q, H, D, ctx, quant, stream):
-    """The outputs: ctx given, made (zeros, so that rows outside every sequence are defined) or left out for the
-    quantized pair."""
+def _context(name, q, M, width, ctx, quant, stream, dev):
+    """The outputs (ctx, its address and pitch, the pair, its addresses): ctx given or made (zeros, so that rows outside
+    every sequence are defined), or the quantized pair."""
     import torch
-    M, dev = q.shape[0], q.device
-    if quant:
-        if ctx is not None:
-            raise E2MIError(f"{name}: either ctx or the quantized pair")
-        return None, *_on(stream, lambda: (torch.zeros((M, H * D), dtype=torch.int8, device=dev),
-                                           torch.zeros((M, H * D // 128), dtype=torch.float32, device=dev)))
-    if ctx is None:
-        ctx = _on(stream, lambda: torch.zeros((M, H * D), dtype=q.dtype, device=dev))
-    if ctx.shape != (M, H * D):
-        raise E2MIError(f"{name}: needs ctx [{M}, {H * D}], got {tuple(ctx.shape)}")
-    _dtype(q, ctx)
-    return ctx, None, None
+    if not quant:
+        if ctx is None:
+            ctx = _new(stream, q.new_zeros, (M, width))
+        return ctx, *_rows(name, ctx, M, width, q.dtype, dev), None, None, None
+    if ctx is not None:
+        raise E2MIError(f"{name}: either ctx or the quantized pair")
+    cq = _new(stream, torch.zeros, (M, width), dtype=torch.int8, device=q.device)
+    cs = _new(stream, torch.zeros, (M, width // 128), dtype=torch.float32, device=q.device)
+    return None, None, 0, (cq, cs), cq.data_ptr(), cs.data_ptr()
 
 
-def _workspace(need, workspace, dev, stream):
-    """The caller's workspace, or a new one of `need` bytes; (tensor, address, bytes)."""
-    import torch
+def _workspace(name, need, workspace, like, stream, dev):
+    """The caller's workspace, or a new one of `need` bytes: (tensor, address, bytes)."""
     if workspace is None:
         if not need:
             return None, None, 0
-        workspace = _on(stream, lambda: torch.empty(need, dtype=torch.uint8, device=dev))
-    elif workspace.device != dev or not workspace.is_contiguous():
-        raise E2MIError(f"needs a contiguous workspace on {dev}")
-    return workspace, _p(workspace), workspace.numel() * workspace.element_size()
+        import torch
+        workspace = _new(stream, torch.empty, need, dtype=torch.uint8, device=like.device)
+        return workspace, workspace.data_ptr(), need
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        raise E2MIError(f"{name}: needs a contiguous workspace on device {dev}")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _ld(t, width):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, dev, *sizes):
+    """e2mi_<name>_workspace_bytes(sizes); the plan also counts the device's compute units, hence dev."""
+    return getattr(load(), f"e2mi_{name}_workspace_bytes")(*sizes)
 
 
 def attention_prefix(q, k, vt, pk, pvt, q_start, q_len, max_q, H, KV, k_start=None, k_len=None, max_k=None, scale=1.0,
@@ -884,48 +909,51 @@ def attention_prefix(q, k, vt, pk, pvt, q_start, q_len, max_q, H, KV, k_start=No
     own keys k [Mk, KV * D] and vt [KV, D, >= Mk] (k None: none), the prefix's pk [P, KV * D] and pvt
     [KV, D, >= P] (None: none); ranges int32 [B] on the device, key ranges those of q unless given. Returns
     ctx [Mq, H * D] (new unless given), or with quant the pair (int8 [Mq, H * D], f32 scales per 128)."""
-    lib = load()
-    D = q.shape[1] // H
-    keys = [t for t in (k, vt, pk, pvt) if t is not None]
-    kind = _dtype(q, *keys)
-    if q.dim() != 2 or q.shape[1] != H * D:
-        raise E2MIError(f"attention_prefix: needs q [rows, {H} heads], got {tuple(q.shape)}")
-    k_start, k_len = q_start if k_start is None else k_start, q_len if k_len is None else k_len
+    name = "attention_prefix"
+    kind, dev = _kind(name, q)
+    Mq, width = q.shape
+    dtype, B, D = q.dtype, q_start.shape[0], width // H
+    pq, lq = _rows(name, q, Mq, H * D, dtype, dev)
+    own, pre = _keys(name, k, vt, KV, D, dtype, dev), _keys(name, pk, pvt, KV, D, dtype, dev)
+    qs, ql = _indices(name, q_start, B, dev), _indices(name, q_len, B, dev)
+    ks = qs if k_start is None else _indices(name, k_start, B, dev)
+    kl = ql if k_len is None else _indices(name, k_len, B, dev)
     max_k = max_q if max_k is None else max_k
-    B, Mq = q_start.shape[0], q.shape[0]
-    _i32(q.device, B, q_start=q_start, q_len=q_len, k_start=k_start, k_len=k_len)
-    own, pre = _keys_of("attention_prefix", k, vt, KV, D), _keys_of("attention_prefix", pk, pvt, KV, D)
-    ctx, cq, cs = _contexts("attention_prefix", q, H, D, ctx, quant, stream)
-    ws, wp, wn = _workspace(lib.e2mi_attention_prefix_workspace_bytes(Mq, own[4], own[3], pre[4], pre[3], B, max_q, max_k, H, KV, D), workspace, q.device,
-                            stream)
-    check(lib.e2mi_attention_prefix(_stream(stream), kind, _p(q), _ld(q, H * D), Mq, *own, *pre, _p(q_start), _p(q_len),
-                                    _p(k_start), _p(k_len), B, max_q, max_k, H, KV, D, scale, int(causal), _p(ctx),
-                                    0 if ctx is None else _ld(ctx, H * D), _p(cq), _p(cs), wp, wn), "attention_prefix")
-    return ctx if ctx is not None else (cq, cs)
+    ctx, pc, lc, pair, cq, cs = _context(name, q, Mq, width, ctx, quant, stream, dev)
+    ws, pw, nw = _workspace(name, _workspace_bytes(name, dev, Mq, own[4], own[3], pre[4], pre[3], B, max_q, max_k, H, KV, D),
+                            workspace, q, stream, dev)
+    check(load().e2mi_attention_prefix(_stream(stream), kind, pq, lq, Mq, *own, *pre, qs, ql, ks, kl, B, max_q, max_k, H, KV, D,
+                                       scale, 1 if causal else 0, pc, lc, cq, cs, pw, nw), name)
+    return pair if quant else ctx
+
+
+def _bounds(name, bounds, B, NB, KV, D, dev):
+    import torch
+    b, s = bounds
+    if b.shape != (B, NB, KV, 2 * D) or s.shape != (B, NB, KV):
+        raise E2MIError(f"{name}: needs bounds [{B}, {NB}, {KV}, {2 * D}] and [{B}, {NB}, {KV}], got {tuple(b.shape)}, {tuple(s.shape)}")
+    if (b.dtype is not torch.int8 or s.dtype is not torch.float32 or b.get_device() != dev or s.get_device() != dev or
+            not b.is_contiguous() or not s.is_contiguous()):
+        raise E2MIError(f"{name}: needs contiguous int8 bounds and float32 scales on device {dev}")
+    return b.data_ptr(), s.data_ptr()
 
 
 def block_bounds(k, k_start, k_len, max_k, KV, bounds=None, stream=None):
     """Bounds of every block of 64 keys (e2mi_block_bounds): (int8 [B, ceil(max_k / 64), KV, 2 * D], f32 [B, .., KV]),
-    new (zeros) unless given."""
+    new unless given. Blocks past a sequence's keys are left as they are."""
     import torch
-    kind = _dtype(k)
-    D, B, NB = k.shape[1] // KV, k_start.shape[0], (max_k + 63) // 64
-    _i32(k.device, B, k_start=k_start, k_len=k_len)
+    name = "block_bounds"
+    kind, dev = _kind(name, k)
+    Mk, width = k.shape
+    D, B, NB = width // KV, k_start.shape[0], (max_k + 63) // 64
+    pk, lk = _rows(name, k, Mk, KV * D, k.dtype, dev)
     if bounds is None:
-        bounds = _on(stream, lambda: (torch.zeros((B, NB, KV, 2 * D), dtype=torch.int8, device=k.device),
-                                      torch.zeros((B, NB, KV), dtype=torch.float32, device=k.device)))
-    _check_bounds("block_bounds", bounds, B, NB, KV, D, k.device)
-    check(load().e2mi_block_bounds(_stream(stream), kind, _p(k), _ld(k, KV * D), k.shape[0], _p(k_start), _p(k_len), B, max_k, KV,
-                                   D, _p(bounds[0]), _p(bounds[1])), "block_bounds")
+        bounds = (_new(stream, torch.empty, (B, NB, KV, 2 * D), dtype=torch.int8, device=k.device),
+                  _new(stream, torch.empty, (B, NB, KV), dtype=torch.float32, device=k.device))
+    pb, ps = _bounds(name, bounds, B, NB, KV, D, dev)
+    check(load().e2mi_block_bounds(_stream(stream), kind, pk, lk, Mk, _indices(name, k_start, B, dev), _indices(name, k_len, B, dev),
+                                   B, max_k, KV, D, pb, ps), name)
     return bounds
-
-
-def _check_bounds(name, bounds, B, NB, KV, D, dev):
-    import torch
-    b, s = bounds
-    if (b.shape != (B, NB, KV, 2 * D) or s.shape != (B, NB, KV) or b.dtype != torch.int8 or s.dtype != torch.float32 or
-            b.device != dev or s.device != dev or not b.is_contiguous() or not s.is_contiguous()):
-        raise E2MIError(f"{name}: needs contiguous bounds int8 [{B}, {NB}, {KV}, {2 * D}] and f32 [{B}, {NB}, {KV}] on {dev}")
 
 
 def block_select(q, bounds, q_start, q_len, k_len, max_q, max_k, H, KV, q_block, n_sel, n_first=0, n_local=0, causal=False,
@@ -933,21 +961,23 @@ def block_select(q, bounds, q_start, q_len, k_len, max_q, max_k, H, KV, q_block,
     """The blocks each block of q_block queries reads (e2mi_block_select) from block_bounds' pair: sel int32
     [B, ceil(max_q / q_block), KV, n_sel], ascending, -1 past the last."""
     import torch
-    lib = load()
-    kind = _dtype(q)
-    D, B, dev = q.shape[1] // H, q_start.shape[0], q.device
-    _i32(dev, B, q_start=q_start, q_len=q_len, k_len=k_len)
-    _check_bounds("block_select", bounds, B, (max_k + 63) // 64, KV, D, dev)
-    shape = (B, (max_q + max(q_block, 1) - 1) // max(q_block, 1), KV, max(n_sel, 0))
+    name = "block_select"
+    kind, dev = _kind(name, q)
+    Mq, width = q.shape
+    D, B = width // H, q_start.shape[0]
+    pq, lq = _rows(name, q, Mq, H * D, q.dtype, dev)
+    pb, ps = _bounds(name, bounds, B, (max_k + 63) // 64, KV, D, dev)
+    if q_block <= 0 or n_sel <= 0:
+        raise E2MIError(f"{name}: needs q_block and n_sel of at least 1 ({q_block}, {n_sel})")
+    shape = (B, (max_q + q_block - 1) // q_block, KV, n_sel)
     if sel is None:
-        sel = _on(stream, lambda: torch.empty(shape, dtype=torch.int32, device=dev))
-    if sel.shape != shape:
-        raise E2MIError(f"block_select: needs sel {shape}, got {tuple(sel.shape)}")
-    _i32(dev, 0, sel=sel)
-    ws, wp, wn = _workspace(lib.e2mi_block_select_workspace_bytes(B, max_q, max_k, KV, q_block), workspace, dev, stream)
-    check(lib.e2mi_block_select(_stream(stream), kind, _p(q), _ld(q, H * D), q.shape[0], _p(bounds[0]), _p(bounds[1]), _p(q_start),
-                                _p(q_len), _p(k_len), B, max_q, max_k, H, KV, D, q_block, n_sel, n_first, n_local, int(causal),
-                                _p(sel), wp, wn), "block_select")
+        sel = _new(stream, torch.empty, shape, dtype=torch.int32, device=q.device)
+    elif sel.shape != shape:
+        raise E2MIError(f"{name}: needs sel {shape}, got {tuple(sel.shape)}")
+    ws, pw, nw = _workspace(name, _workspace_bytes(name, dev, B, max_q, max_k, KV, q_block), workspace, q, stream, dev)
+    check(load().e2mi_block_select(_stream(stream), kind, pq, lq, Mq, pb, ps, _indices(name, q_start, B, dev),
+                                   _indices(name, q_len, B, dev), _indices(name, k_len, B, dev), B, max_q, max_k, H, KV, D, q_block,
+                                   n_sel, n_first, n_local, 1 if causal else 0, _indices(name, sel, 0, dev), pw, nw), name)
     return sel
 
 
@@ -955,24 +985,23 @@ def attention_blocks(q, k, vt, sel, q_start, q_len, k_start, k_len, max_q, max_k
                      quant=False, workspace=None, stream=None):
     """Attention over the listed blocks of 64 keys (e2mi_attention_blocks): sel as block_select gives it. Returns as
     attention_prefix."""
-    lib = load()
-    D, B, Mq, dev = q.shape[1] // H, q_start.shape[0], q.shape[0], q.device
-    kind = _dtype(q, k, vt)
-    if q.dim() != 2 or q.shape[1] != H * D:
-        raise E2MIError(f"attention_blocks: needs q [rows, {H} heads], got {tuple(q.shape)}")
-    if sel.dim() != 4 or sel.shape[:3] != (B, (max_q + max(q_block, 1) - 1) // max(q_block, 1), KV):
-        raise E2MIError(f"attention_blocks: needs sel [B, query blocks, {KV}, n], got {tuple(sel.shape)}")
-    _i32(dev, B, q_start=q_start, q_len=q_len, k_start=k_start, k_len=k_len)
-    _i32(dev, 0, sel=sel)
-    own = _keys_of("attention_blocks", k, vt, KV, D)
-    ctx, cq, cs = _contexts("attention_blocks", q, H, D, ctx, quant, stream)
+    name = "attention_blocks"
+    kind, dev = _kind(name, q)
+    Mq, width = q.shape
+    dtype, B, D = q.dtype, q_start.shape[0], width // H
+    pq, lq = _rows(name, q, Mq, H * D, dtype, dev)
+    own = _keys(name, k, vt, KV, D, dtype, dev)
+    if q_block <= 0 or sel.dim() != 4 or sel.shape[:3] != (B, (max_q + q_block - 1) // q_block, KV):
+        raise E2MIError(f"{name}: needs q_block of at least 1 and sel [{B}, query blocks, {KV}, n], got {q_block}, {tuple(sel.shape)}")
     n_sel = sel.shape[3]
-    ws, wp, wn = _workspace(lib.e2mi_attention_blocks_workspace_bytes(Mq, own[4], own[3], B, max_q, H, KV, D, q_block, n_sel), workspace, dev,
-                            stream)
-    check(lib.e2mi_attention_blocks(_stream(stream), kind, _p(q), _ld(q, H * D), Mq, *own, _p(q_start), _p(q_len), _p(k_start),
-                                    _p(k_len), B, max_q, max_k, H, KV, D, q_block, _p(sel), n_sel, scale, int(causal), _p(ctx),
-                                    0 if ctx is None else _ld(ctx, H * D), _p(cq), _p(cs), wp, wn), "attention_blocks")
-    return ctx if ctx is not None else (cq, cs)
+    ctx, pc, lc, pair, cq, cs = _context(name, q, Mq, width, ctx, quant, stream, dev)
+    ws, pw, nw = _workspace(name, _workspace_bytes(name, dev, Mq, own[4], own[3], B, max_q, H, KV, D, q_block, n_sel), workspace, q,
+                            stream, dev)
+    check(load().e2mi_attention_blocks(_stream(stream), kind, pq, lq, Mq, *own, _indices(name, q_start, B, dev),
+                                       _indices(name, q_len, B, dev), _indices(name, k_start, B, dev), _indices(name, k_len, B, dev),
+                                       B, max_q, max_k, H, KV, D, q_block, _indices(name, sel, 0, dev), n_sel, scale,
+                                       1 if causal else 0, pc, lc, cq, cs, pw, nw), name)
+    return pair if quant else ctx
 
 
 # ---- model container and encoder engine
