@@ -79,45 +79,6 @@ __device__ inline typename Half8<T>::type load8(const uint16_t *p) {
 
 __device__ inline int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
 
-// Writes DW dims of a row's context from dim0 on (a lane holds dims 32 t + 8 g + 4 half + 0..3 of its row, o already
-// divided by the sum): 16-bit rows, and per 128 dims the quantized pair of the O projection.
-template <class T, int D, int DW = D>
-__device__ __forceinline__ void write_row(const KeysArgs &a, const f16v (&o)[DW / 32], int64_t m, int h, int half, int dim0 = 0) {
-    typedef T v4 __attribute__((ext_vector_type(4)));
-    if (a.ctx) {
-        T *y = (T *)a.ctx + m * a.ldc + (int64_t)h * D + dim0 + 4 * half;
-#pragma unroll
-        for (int t = 0; t < DW / 32; t++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const v4 v = {(T)o[t][4 * g], (T)o[t][4 * g + 1], (T)o[t][4 * g + 2], (T)o[t][4 * g + 3]};
-                *(v4 *)(y + 32 * t + 8 * g) = v;
-            }
-    }
-    if constexpr (D % 128 == 0) {
-        if (a.cq) {
-            const int64_t row = m * a.H + h;
-#pragma unroll
-            for (int blk = 0; blk < DW / 128; blk++) {
-                float am = 0.f;
-#pragma unroll
-                for (int t = 4 * blk; t < 4 * blk + 4; t++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) am = fmaxf(am, fabsf(o[t][r]));
-                am = fmaxf(am, xor_lane<32>(am));
-                const QScale qs = qscale(am);
-#pragma unroll
-                for (int t = 4 * blk; t < 4 * blk + 4; t++)
-#pragma unroll
-                    for (int g = 0; g < 4; g++)
-                        *(uint32_t *)(a.cq + row * D + dim0 + 32 * t + 8 * g + 4 * half) =
-                            pack4_magic(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3], qs.inv);
-                if (half == 0) a.cs[row * (D / 128) + dim0 / 128 + blk] = qs.sc;
-            }
-        }
-    }
-}
-
 // The blocks of a selection list that hold keys this tile may see, compacted in list order into LDS; returns
 // their number (every thread of the workgroup). blocks: those below it may be read.
 __device__ inline int read_list(const int32_t *sel, int n_sel, int blocks, int *list, int *count) {
@@ -211,20 +172,10 @@ __device__ inline KeySet set_of(const KeysArgs &a, bool pre) {
     return s;
 }
 
-// Leaves a row's share for k_keys_merge: no key: nothing but the maximum says so; a NaN sum (NaN rows) takes the
-// whole row with it.
-template <int D, int DW = D>
-__device__ __forceinline__ void write_share(const KeysArgs &a, const f16v (&o)[DW / 32], float mx, float sum, int part, int64_t m,
-                                            int h, int half, int dim0 = 0) {
-    const int64_t row = ((int64_t)(a.part0 + part) * a.Mq + m) * a.H + h;
-    if (half == 0 && dim0 == 0) *(float2 *)(a.part_ml + row * 2) = make_float2(sum == sum ? mx : INFINITY, sum);
-    if (sum == 0.f) return;
-    float *y = a.part_o + row * D + dim0 + 4 * half;
-#pragma unroll
-    for (int i = 0; i < DW / 32; i++)
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-            *(float4 *)(y + 32 * i + 8 * g) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+// What is left of a share for k_keys_merge beside its context: without keys the sum is 0 (and no context is written); a NaN
+// sum (NaN rows) takes the whole row with it.
+__device__ inline void write_share(const KeysArgs &a, int64_t row, float mx, float sum) {
+    *(float2 *)(a.part_ml + row * 2) = make_float2(sum == sum ? mx : INFINITY, sum);
 }
 
 // Few rows: 16 a workgroup, whose waves take every WV-th key tile of 32 and are joined through LDS. Bound by HBM, hence by
@@ -430,7 +381,7 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
         const int64_t m = (int64_t)k.qs + k.tok0 + rc / a.G;
         if (a.part_o) {
             const int64_t to = ((int64_t)(a.part0 + k.part) * a.Mq + m) * a.H + h;
-            if (live && d == 0) *(float2 *)(a.part_ml + to * 2) = make_float2(sum == sum ? mall : INFINITY, sum);
+            if (live && d == 0) write_share(a, to, mall, sum);
             if (live && sum != 0.f) *(f4v *)(a.part_o + to * D + d) = v;
             continue;
         }
@@ -469,7 +420,11 @@ struct WideTile {
     static constexpr int KB = DS == 1 ? 2 : 1;      // K buffers
     static constexpr int kV = KB * kTile;           // V^T's two
     static constexpr int kX = kV + 2 * kTile;       // the exchange: 4 KB a wave
-    static constexpr int bytes(int nw) { return kX + (DS > 1 ? nw * DS * 4096 : 0); }
+    static constexpr int PITCH = 68;                // floats of a row of 64 dims on its way out
+    static constexpr int bytes(int nw) {
+        const int walk = kX + (DS > 1 ? nw * DS * 4096 : 0), out = nw * DS * 32 * PITCH * 4;
+        return walk > out ? walk : out;
+    }
 };
 // K and V^T fragments are read this many MFMAs ahead of their use
 constexpr int kAhead = 3;
@@ -657,21 +612,85 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
             if (i + kAhead < 2 * NO) vr[i % kAhead] = vfrag(i + kAhead);
         }
     }
+    // The epilogue: 64 dims at a time through LDS of the wave's own, so that 16 lanes write a row's run of 256 bytes (128 in
+    // 16-bit types; 64 of quantized bytes) instead of every lane 8 bytes of a row of its own
+    __syncthreads();  // the tiles are read
+    if (!active) return;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    constexpr int PITCH = L::PITCH;
     const float lsum = lrun + xor_lane<32>(lrun);
+    float *sx = (float *)wide_smem + wu * (32 * PITCH);
     int l = lane;
     asm volatile("" : "+v"(l));  // the row again, not kept in registers through the loop
-    if (r1 + (l & 31) >= k.rows) return;
     int tok, h;
     row_of(l, tok, h);
-    const int64_t m = (int64_t)k.qs + tok;
-    if (a.part_o) {
-        write_share<D, DW>(a, o, mrun, lsum, k.part, m, h, l >> 5, dim0);
-        return;
+    const int m = k.qs + tok;
+    const bool share = a.part_o != nullptr;
+    float scale = 1.f;  // of the values written
+    if (share) {
+        if (l < 32 && r1 + l < k.rows && dim0 == 0) write_share(a, ((int64_t)(a.part0 + k.part) * a.Mq + m) * a.H + h, mrun, lsum);
+    } else {
+        scale = lsum == 0.f ? 0.f : __fdiv_rn(1.f, lsum);
     }
-    const float inv = lsum == 0.f ? 0.f : __fdiv_rn(1.f, lsum);
 #pragma unroll
-    for (int i = 0; i < NO; i++) o[i] *= inv;
-    write_row<T, D, DW>(a, o, m, h, l >> 5, dim0);
+    for (int i = 0; i < NO; i++) o[i] *= scale;
+    const int quad = l & 15, sub = l >> 4;
+    const uint64_t some = __ballot(lsum != 0.f);
+    if (share || a.ctx) {
+#pragma unroll
+        for (int p = 0; p < DW / 64; p++) {
+            float *y = sx + (l & 31) * PITCH + 4 * (l >> 5);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    *(float4 *)(y + 32 * t + 8 * g) =
+                        make_float4(o[2 * p + t][4 * g], o[2 * p + t][4 * g + 1], o[2 * p + t][4 * g + 2], o[2 * p + t][4 * g + 3]);
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                const int row = 4 * x + sub, mr = __shfl(m, row), hr = __shfl(h, row), d = dim0 + 64 * p + 4 * quad;
+                const float4 v = *(const float4 *)(sx + row * PITCH + 4 * quad);
+                if (r1 + row >= k.rows) continue;
+                if (share) {
+                    if (some >> row & 1) *(float4 *)(a.part_o + (((int64_t)(a.part0 + k.part) * a.Mq + mr) * a.H + hr) * D + d) = v;
+                } else {
+                    const T4 z = {(T)v.x, (T)v.y, (T)v.z, (T)v.w};
+                    *(T4 *)((T *)a.ctx + mr * a.ldc + (int64_t)hr * D + d) = z;
+                }
+            }
+        }
+    }
+    if constexpr (D % 128 == 0) {
+        if (!share && a.cq) {
+#pragma unroll
+            for (int blk = 0; blk < DW / 128; blk++) {
+                float am = 0.f;
+#pragma unroll
+                for (int t = 4 * blk; t < 4 * blk + 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) am = fmaxf(am, fabsf(o[t][e]));
+                am = fmaxf(am, xor_lane<32>(am));
+                const QScale q = qscale(am);
+                if (l < 32 && r1 + l < k.rows) a.cs[((int64_t)m * a.H + h) * (D / 128) + dim0 / 128 + blk] = q.sc;
+                uint32_t *y = (uint32_t *)sx + (l & 31) * PITCH + (l >> 5);
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const f16v &z = o[4 * blk + t];
+                        y[8 * t + 2 * g] = pack4_magic(z[4 * g], z[4 * g + 1], z[4 * g + 2], z[4 * g + 3], q.inv);
+                    }
+#pragma unroll
+                for (int x = 0; x < 4; x++) {  // 8 lanes a row: 16 bytes each
+                    const int row = 8 * x + (l >> 3), mr = __shfl(m, row), hr = __shfl(h, row);
+                    const uint4 v = *(const uint4 *)((uint32_t *)sx + row * PITCH + 4 * (l & 7));
+                    if (r1 + row >= k.rows) continue;
+                    uint2 *z = (uint2 *)(a.cq + ((int64_t)mr * a.H + hr) * D + dim0 + 128 * blk + 16 * (l & 7));
+                    z[0] = make_uint2(v.x, v.y), z[1] = make_uint2(v.z, v.w);
+                }
+            }
+        }
+    }
 }
 
 // V^T rows of any pitch and address, copied to a pitch that 16-byte loads take.
@@ -688,17 +707,20 @@ __global__ __launch_bounds__(256) void k_pad_rows(uint16_t *y, int64_t ldy, cons
     }
 }
 
-// Joins the shares of a row: a wave a row, lane p holding the maxima and sums of shares p and p + 64, then D / 64 dims a
-// lane, eight shares' contexts in flight.
-template <class T, int D>
+// Joins the shares of a row. SPLIT 1: a wave a row, four rows a workgroup; SPLIT 4: four waves a row, a quarter of the
+// shares each, met in LDS (few rows: a wave a row would leave most of the device idle). Lane p holds the maxima and
+// sums of shares p and p + 64, then D / 64 dims, eight shares' contexts in flight.
+template <class T, int D, int SPLIT>
 __global__ __launch_bounds__(256) void k_keys_merge(KeysArgs a) {
     constexpr int VW = D / 64;
     typedef float vf __attribute__((ext_vector_type(VW)));
     typedef T vt __attribute__((ext_vector_type(VW)));
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, b = blockIdx.z;
+    __shared__ vf s_o[SPLIT > 1 ? 3 * 64 : 1];
+    const int lane = threadIdx.x & 63, b = blockIdx.z;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int qs, nq;
     if (!row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, qs, nq)) return;
-    const int64_t i = (int64_t)blockIdx.x * 4 + w;
+    const int64_t i = SPLIT > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + w;
     if (i >= (int64_t)nq * a.H) return;
     const int64_t row = (int64_t)qs * a.H + i, pitch = (int64_t)a.Mq * a.H;
     float mp[2], wp[2], sum = 0.f;
@@ -718,19 +740,27 @@ __global__ __launch_bounds__(256) void k_keys_merge(KeysArgs a) {
         wp[x] = wp[x] == 0.f ? 0.f : f;  // a share without keys left no context
     }
     sum = group_sum<64>(sum);
+    const int first = SPLIT > 1 ? a.all_parts * w / 4 : 0, end = SPLIT > 1 ? a.all_parts * (w + 1) / 4 : a.all_parts;
     vf o = {};
     const float *from = a.part_o + row * D + lane * VW;
-    for (int p0 = 0; p0 < a.all_parts; p0 += 8) {
+    for (int p0 = first; p0 < end; p0 += 8) {
         vf v[8];
 #pragma unroll
-        for (int x = 0; x < 8; x++) v[x] = *(const vf *)(from + min(p0 + x, a.all_parts - 1) * pitch * D);
+        for (int x = 0; x < 8; x++) v[x] = *(const vf *)(from + min(p0 + x, end - 1) * pitch * D);
 #pragma unroll
         for (int x = 0; x < 8; x++) {
             const int p = p0 + x;
             const float f = __builtin_bit_cast(float, p < 64 ? __builtin_amdgcn_readlane(__builtin_bit_cast(int, wp[0]), p & 63)
                                                              : __builtin_amdgcn_readlane(__builtin_bit_cast(int, wp[1]), p & 63));
-            if (p < a.all_parts && f != 0.f) o += v[x] * f;
+            if (p < end && f != 0.f) o += v[x] * f;
         }
+    }
+    if constexpr (SPLIT > 1) {
+        if (w) s_o[(w - 1) * 64 + lane] = o;
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int x = 0; x < 3; x++) o += s_o[x * 64 + lane];
     }
     const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
     o *= inv;
@@ -773,23 +803,26 @@ struct KeysPlan {
     int all() const { return (apart ? pre.parts : 0) + rows.parts; }
 };
 
-// Shares for `groups` workgroups whose longest walk is `tiles` key tiles of 32: enough to give every CU two
-// workgroups, at least `least` tiles each.
-static int key_shares(int64_t groups, int64_t tiles, int least, int most) {
+// Shares for `groups` workgroups whose longest walk is `tiles` key tiles of 32: enough to give every CU `per` workgroups, at
+// least `least` tiles each.
+static int key_shares(int64_t groups, int64_t tiles, int per, int least, int most) {
     if (groups < 1) return 1;
-    const int64_t want = (2L * num_cus() + groups - 1) / groups;
+    const int64_t want = ((int64_t)per * num_cus() + groups - 1) / groups;
     int64_t n = want < tiles / least ? want : tiles / least;
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
 }
 
 // groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles
-static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int most) {
+static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int most) {
     RowsPlan p;
     p.nw = rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
+    // one launch of few rows that cannot fill the device even in shares: half as many rows a workgroup
+    if (p.nw == 4 && (rows + 127) / 128 * count * most < num_cus()) p.nw = 2;
     const int R = p.nw ? 32 * p.nw : 16;
     p.tiles = (rows + R - 1) / R;
-    p.parts = key_shares(p.tiles * count, tiles, 8, most);
+    // k_keys_few fills a CU's LDS from head_dim 256 on
+    p.parts = key_shares(p.tiles * count, tiles, p.nw || D < 256 ? 2 : 1, p.nw ? 8 : 4, most);
     return p;
 }
 
@@ -804,8 +837,8 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
     const int64_t rows = (int64_t)max_q * G;
     // sequences of less than a tile share the prefix's tiles
     p.apart = B > 1 && P > 0 && rows < 32;
-    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, kMaxKeyParts / 2);
-    p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), p.apart ? kMaxKeyParts / 2 : kMaxKeyParts);
+    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, D, kMaxKeyParts / 2);
+    p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), D, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts);
     if (needs_copy(pre)) p.pad_pre = pad_bytes(P, KV, D);
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
@@ -814,7 +847,7 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
 static KeysPlan plan_blocks(const KeySet &own, int B, int max_q, int H, int KV, int D, int q_block, int n_sel) {
     KeysPlan p;
     const int64_t NQ = ((int64_t)max_q + q_block - 1) / q_block;
-    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, kMaxKeyParts);
+    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, D, kMaxKeyParts);
     p.rows.tiles *= NQ;
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
@@ -879,7 +912,11 @@ static int run_keys(hipStream_t st, KeysArgs a, const KeysPlan &p, void *workspa
     a.mode = a.sel ? kSelected : kOwnRows;
     if (launch_rows<T, D>(st, a, p.rows, a.B)) return -1;
     if (a.all_parts == 1) return 0;
-    hipLaunchKernelGGL((k_keys_merge<T, D>), dim3((unsigned)(((int64_t)a.max_q * a.H + 3) / 4), 1, a.B), dim3(256), 0, st, a);
+    const int64_t rows = (int64_t)a.max_q * a.H;
+    if (rows * a.B <= 4L * num_cus())
+        hipLaunchKernelGGL((k_keys_merge<T, D, 4>), dim3((unsigned)rows, 1, a.B), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_keys_merge<T, D, 1>), dim3((unsigned)((rows + 3) / 4), 1, a.B), dim3(256), 0, st, a);
     return check_hip(hipGetLastError(), "attention merge launch");
 }
 

@@ -203,8 +203,8 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t u = raw[s][2 * e], v = raw[s][2 * e + 1];
-                    const uint32_t x = pack4(qbyte(value_of<T>((uint16_t)u), q.inv), qbyte(value_of<T>((uint16_t)(u >> 16)), q.inv),
-                                             qbyte(value_of<T>((uint16_t)v), q.inv), qbyte(value_of<T>((uint16_t)(v >> 16)), q.inv));
+                    const uint32_t x = pack4_magic(value_of<T>((uint16_t)u), value_of<T>((uint16_t)(u >> 16)), value_of<T>((uint16_t)v),
+                                                   value_of<T>((uint16_t)(v >> 16)), q.inv);
                     const uint32_t neg = (uint32_t)byte_lanes_negative(x);
                     up[s][e] = (int)(x & ~neg);
                     down[s][e] = (int)(x & neg);
@@ -319,6 +319,7 @@ template <int W, int RPL>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_block_top(SelectArgs a, int64_t lists) {
     constexpr int WG = W > 4 ? W : 4;  // waves a workgroup
     __shared__ int s_n[W > 1 ? 2 : 1][W];
+    __shared__ int s_n3[W > 1 ? 2 : 1][W][3];
     __shared__ uint32_t s_ends[2][W];
     const int lane = threadIdx.x & 63, w = W > 1 ? threadIdx.x >> 6 : 0;
     const int64_t id = (int64_t)blockIdx.x * (WG / W) + (W > 1 ? 0 : threadIdx.x >> 6);
@@ -360,6 +361,13 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_block_top(SelectArgs a
             return all;
         }
     };
+    auto totals = [&](int &x, int &y, int &z) {  // three sums over the list's waves
+        if (lane < 3) s_n3[flip][w][lane] = lane == 0 ? x : lane == 1 ? y : z;
+        __syncthreads();
+        x = y = z = 0;
+        for (int i = 0; i < W; i++) x += s_n3[flip][i][0], y += s_n3[flip][i][1], z += s_n3[flip][i][2];
+        flip ^= 1;
+    };
     auto count = [&](uint32_t from) {
         int c = 0;
 #pragma unroll
@@ -384,11 +392,13 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_block_top(SelectArgs a
         }
         const int bits = hi == lo ? 0 : 32 - __clz(hi ^ lo);
         cut = bits < 32 ? hi >> bits << bits : 0;
-        for (int bit = bits - 1; bit >= 0; bit--) {
-            const uint32_t c = cut | (1u << bit);
-            const int n = total(count(c), before);
-            if (n >= a.n_sel) cut = c;
-            if (n == a.n_sel) break;
+        for (int bit = bits - 1; bit >= 0; bit -= 2) {  // two bits a step: three counts in flight
+            const uint32_t one = bit > 0 ? 1u << (bit - 1) : 0u, two = 1u << bit;
+            const int c1 = count(cut + one), c2 = count(cut + two), c3 = count(cut + two + one);
+            int n1 = c1, n2 = c2, n3 = c3;
+            if constexpr (W > 1) totals(n1, n2, n3);
+            cut += n3 >= a.n_sel ? two + one : n2 >= a.n_sel ? two : n1 >= a.n_sel ? one : 0u;
+            if (n1 == a.n_sel || n2 == a.n_sel || n3 == a.n_sel) break;
         }
         above = total(count(cut + 1), before);
     } else if (forced >= a.n_sel) {
@@ -533,7 +543,8 @@ extern "C" int e2mi_block_select(e2mi_stream stream, int dtype, const uint16_t *
     const unsigned n = (unsigned)lists;
     // a wave a list, keys in registers; past 1024 blocks four where the lists are too few to fill the device
     const bool few = lists < 4L * num_cus();
-    if (a.NB <= 512) hipLaunchKernelGGL((k_block_top<1, 8>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
+    if (a.NB <= 256 || (a.NB <= 512 && !few)) hipLaunchKernelGGL((k_block_top<1, 8>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
+    else if (a.NB <= 1024 && few) hipLaunchKernelGGL((k_block_top<4, 4>), dim3(n), dim3(256), 0, st, a, lists);
     else if (a.NB <= 1024) hipLaunchKernelGGL((k_block_top<1, 16>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
     else if (a.NB <= 2048 && few) hipLaunchKernelGGL((k_block_top<4, 8>), dim3(n), dim3(256), 0, st, a, lists);
     else if (a.NB <= 2048) hipLaunchKernelGGL((k_block_top<1, 32>), dim3((n + 3) / 4), dim3(256), 0, st, a, lists);
