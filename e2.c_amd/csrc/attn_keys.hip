@@ -426,11 +426,47 @@ struct WideTile {
         return walk > out ? walk : out;
     }
 };
+// The work of a workgroup of a grid that is a multiple of 64. Runs of 8 consecutive tiles of a sequence, which read the same
+// keys, go to one XCD and its L2 (workgroup i runs on XCD i % 8); the runs are dealt out in turn, their order turned
+// from one round of 8 to the next, because the tiles past a short sequence's end come in runs too: dealt as one range an
+// XCD, 64 texts of 64 to 512 tokens kept the CUs busy half of the time.
+__device__ inline int spread(int i) {
+    const int xcd = i & 7, slot = i >> 3, round = slot >> 3;
+    return (round * 8 + ((xcd + round + (round >> 2)) & 7)) * 8 + (slot & 7);
+}
+// Work item `item` of those that have rows, over sequences, kv heads and tiles of R rows in that order (a wave's lanes add up
+// 64 sequences at a time): with a grid of max_q rows a sequence, the tiles past short sequences' ends would leave
+// their XCDs idle. False past the last item.
+constexpr int kFindMost = 512;  // sequences; beyond, the sums take longer than idle workgroups
+__device__ inline bool find_tile(const KeysArgs &a, int R, int item, int &b, int &kvh, int &tile) {
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        int s, nq, n = 0;
+        if (b0 + lane < a.B && row_range(a.q_start, a.q_len, b0 + lane, a.max_q, a.Mq, s, nq))
+            n = a.mode == kSelected ? (nq + a.q_block - 1) / a.q_block * ((a.q_block * a.G + R - 1) / R) : (nq * a.G + R - 1) / R;
+        n *= a.KV;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(sum, o);
+            if (lane >= o) sum += v;
+        }
+        const int all = __builtin_amdgcn_readlane(sum, 63);
+        if (item < all) {
+            const int l = __builtin_ctzll(__ballot(sum > item));
+            const int mine = __builtin_amdgcn_readlane(n, l), at = item - (__builtin_amdgcn_readlane(sum, l) - mine), per = mine / a.KV;
+            b = b0 + l, kvh = at / per, tile = at % per;
+            return true;
+        }
+        item -= all;
+    }
+    return false;
+}
 // K and V^T fragments are read this many MFMAs ahead of their use
 constexpr int kAhead = 3;
 
 template <class T, int D, int NW>
-__global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(KeysArgs a, int tiles) {
+__global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(KeysArgs a, int tiles, int total) {
     typedef typename Half8<T>::type V8;
     using L = WideTile<D>;
     constexpr int DS = L::DS, WV = NW * DS, DW = D / DS;  // waves, dims of a wave
@@ -443,14 +479,20 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
     const int wu = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wu / DS, dim0 = wu % DS * DW;
     int *list = (int *)(wide_smem + L::bytes(NW));
-    // consecutive tiles of a sequence read the same keys: they go to one XCD and its L2
-    int id = xcd_swizzle(blockIdx.x, gridDim.x);
+    int id = spread(blockIdx.x);
+    if (id >= total) return;
     const int part = id % a.parts;
     id /= a.parts;
-    const int tile = id % tiles;
-    id /= tiles;
+    int b, kvh, tile;
+    if (a.B > 1 && a.B <= kFindMost && a.mode != kAllRows) {
+        if (!find_tile(a, 32 * NW, id, b, kvh, tile)) return;
+    } else {
+        tile = id % tiles;
+        id /= tiles;
+        kvh = id % a.KV, b = id / a.KV;
+    }
     Walk k;
-    if (!start_walk<32 * NW>(a, id % a.KV, id / a.KV, tile, part, list, &s_count, k)) return;
+    if (!start_walk<32 * NW>(a, kvh, b, tile, part, list, &s_count, k)) return;
     const int r1 = k.r0 + 32 * group;     // the group's first row
     const bool active = r1 < k.rows;      // a wave without rows loads its share of the tiles only
     auto row_of = [&](int l, int &tok, int &h) {
@@ -478,34 +520,45 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
     const int lr = lane / LPR, lc = lane % LPR;
     const int vchunk = (lane & 3) ^ ((lane >> 4) & 3);
     // A tile's loads: load j of a wave takes K rows RPI x .. + RPI - 1 or V^T rows 16 x .. + 15, x = NLW wave + j.
-    // Descriptors start at the load's first row, so 32 bits hold every offset at any length of the cache.
+    // Descriptors start at the tile's first key, so 32 bits hold every offset at any length of the cache.
+    struct Range {
+        uint64_t k, v;      // addresses of its first key in this kv head; V^T: this wave's first row
+        uint32_t ldk, ldv;  // bytes
+    };
+    auto range_of = [&](const KeySet &s, int first) {
+        Range r;
+        r.k = (uint64_t)(s.k + (int64_t)first * s.ldk + (int64_t)k.kvh * D);
+        r.v = (uint64_t)(s.vt + ((int64_t)k.kvh * D + 16 * NLW * wu) * s.ldv + first);
+        r.ldk = (uint32_t)s.ldk * 2, r.ldv = (uint32_t)s.ldv * 2;
+        return r;
+    };
+    const Range own = range_of(a.own, k.ks), pre = range_of(a.pre, 0);
     struct Fetch {
-        const uint16_t *k, *v;
-        uint32_t ldk, ldv, bytes;  // pitches in bytes; K's range
+        uint64_t k, v;
+        uint32_t ldk, ldv, bytes;  // K's range
         uint32_t ko, vo;           // lane offsets
     };
     auto fetch_of = [&](const KeyTile &kt) {
-        const KeySet src = set_of(a, kt.pre);
-        const int64_t row = (kt.pre ? 0 : k.ks) + kt.key0;
         Fetch f;
-        f.k = src.k + row * src.ldk + (int64_t)k.kvh * D;
-        f.v = src.vt + ((int64_t)k.kvh * D + 16 * NLW * wu) * src.ldv + row;
-        f.ldk = (uint32_t)src.ldk * 2, f.ldv = (uint32_t)src.ldv * 2;
+        f.ldk = kt.pre ? pre.ldk : own.ldk, f.ldv = kt.pre ? pre.ldv : own.ldv;
+        f.k = (kt.pre ? pre.k : own.k) + (uint64_t)(uint32_t)kt.key0 * f.ldk;
+        f.v = (kt.pre ? pre.v : own.v) + 2 * (uint64_t)(uint32_t)kt.key0;
         f.bytes = kt.n ? (uint32_t)(kt.n - 1) * f.ldk + 2 * D : 0;
         f.ko = (uint32_t)swap23(lr) * f.ldk;
         f.vo = 8 * vchunk < kt.n ? (uint32_t)(lane >> 2) * f.ldv + (uint32_t)vchunk * 16 : 0x80000000u;
         return f;
     };
+    const uint32_t kchunk = (uint32_t)((lc ^ (lr & 7)) << 4);
     auto load_k = [&](const Fetch &f, int buf, int j) {
         const int x = NLW * wu + j, i = RPI * x;
         if (NL % WV && x >= NL) return;
-        // a row past the range reads as zero: the lane offset lies past the descriptor's end
-        dma16_nc(rsrc_words(f.k, f.bytes), lds0 + (uint32_t)(buf * L::kTile + i * (2 * D)),
-                 f.ko + (uint32_t)((lc ^ ((i + lr) & 7)) << 4), here((uint32_t)swap23(i) * f.ldk));
+        // row i + lr: chunk lc ^ ((i + lr) & 7). A row past the range reads as zero: its offset lies past the descriptor's end
+        dma16_nc(rsrc_words((const void *)f.k, f.bytes), lds0 + (uint32_t)(buf * L::kTile + i * (2 * D)),
+                 f.ko + (kchunk ^ here((uint32_t)((i & 7) << 4))), here((uint32_t)swap23(i) * f.ldk));
     };
     auto load_v = [&](const Fetch &f, int buf, int j) {
         if (NL % WV && NLW * wu + j >= NL) return;
-        const v4u rs = rsrc_words((const void *)here((uint64_t)f.v + (uint64_t)(16 * j) * f.ldv), 0x7fffffffu);
+        const v4u rs = rsrc_words((const void *)here(f.v + (uint64_t)(16 * j) * f.ldv), 0x7fffffffu);
         dma16_nc(rs, lds0 + (uint32_t)(L::kV + buf * L::kTile + (NLW * wu + j) * 1024), f.vo, 0);
     };
 
@@ -532,11 +585,9 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
         // reads of the buffer that the next loads refill
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        const bool more = t + 1 < k.t1;
-        if (more) {
-            next = key_tile(a, k, list, t + 1);
-            f = fetch_of(next);
-        }
+        // the next tile; after the last one that again, which nobody reads, so that no branch parts the loads from the MFMAs
+        next = key_tile(a, k, list, min(t + 1, k.t1 - 1));
+        f = fetch_of(next);
         unsigned char *sk = wide_smem + kbuf * L::kTile, *sv = wide_smem + buf * L::kTile;
         if (now.n & 7) {  // values past the range in its last chunk (of any bits) become 0
             for (int d = tid; d < D; d += 64 * WV) {
@@ -549,6 +600,11 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
         }
         const bool work = active && now.n > 0;
         f16v st = (f16v){};
+        constexpr int NF = DS == 1 ? 2 * NLW : NLW;  // loads requested here: V^T's, then K's
+        auto request = [&](int j) {
+            if (j < NLW) load_v(f, buf ^ 1, j);
+            else load_k(f, buf ^ 1, j - NLW);
+        };
         if (work) {
             V8 kr[kAhead];
             auto kfrag = [&](int s) { return *(const V8 *)(sk + (krd ^ (uint32_t)((s & 3) << 5)) + (s >> 2) * 128); };
@@ -558,27 +614,21 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
             for (int s = 0; s < NQ; s++) {
                 st = Half8<T>::mma(kr[s % kAhead], qf[s], st);
                 if (s + kAhead < NQ) kr[s % kAhead] = kfrag(s + kAhead);
-                if ((s & 1) && more) {
-                    if ((s >> 1) < NLW) load_v(f, buf ^ 1, s >> 1);
-                    else if (DS == 1 && (s >> 1) < 2 * NLW) load_k(f, buf ^ 1, (s >> 1) - NLW);
-                }
-            }
-        }
-        if (more) {  // what the MFMAs above had no room for
 #pragma unroll
-            for (int j = 0; j < NLW; j++) {
-                if (!work || j >= NQ / 2) load_v(f, buf ^ 1, j);
-                if (DS == 1 && (!work || NLW + j >= NQ / 2)) load_k(f, buf ^ 1, j);
+                for (int j = s * NF / NQ; j < (s + 1) * NF / NQ; j++) request(j);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NF; j++) request(j);
         }
         if constexpr (DS == 2) {
             float4 *x = (float4 *)(wide_smem + L::kX) + wu * 256 + lane;
 #pragma unroll
             for (int i = 0; i < 4; i++) x[64 * i] = make_float4(st[4 * i], st[4 * i + 1], st[4 * i + 2], st[4 * i + 3]);
             lds_barrier();  // the K tile is read: its buffer takes the next one
-            if (more)
 #pragma unroll
-                for (int j = 0; j < NLW; j++) load_k(f, 0, j);
+            for (int j = 0; j < NLW; j++) load_k(f, 0, j);
             const float4 *y = (const float4 *)(wide_smem + L::kX) + (wu ^ 1) * 256 + lane;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -610,11 +660,13 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
         for (int i = 0; i < 2 * NO; i++) {
             o[i >> 1] = Half8<T>::mma(vr[i % kAhead], pb[i & 1], o[i >> 1]);
             if (i + kAhead < 2 * NO) vr[i % kAhead] = vfrag(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     // The epilogue: 64 dims at a time through LDS of the wave's own, so that 16 lanes write a row's run of 256 bytes (128 in
     // 16-bit types; 64 of quantized bytes) instead of every lane 8 bytes of a row of its own
-    __syncthreads();  // the tiles are read
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // the tiles are read, and no load is on its way to them
     if (!active) return;
     typedef T T4 __attribute__((ext_vector_type(4)));
     constexpr int PITCH = L::PITCH;
@@ -859,11 +911,12 @@ static size_t part_bytes(const KeysPlan &p, int Mq, int H, int D) {
 static size_t workspace_of(const KeysPlan &p, int Mq, int H, int D) { return part_bytes(p, Mq, H, D) + p.pad_pre + p.pad_own; }
 
 template <class T, int D, int NW>
-static int launch_wide(hipStream_t st, const KeysArgs &a, int64_t tiles, int64_t grid) {
+static int launch_wide(hipStream_t st, const KeysArgs &a, int64_t tiles, int64_t total) {
     const size_t lds = WideTile<D>::bytes(NW) + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
     static LdsAllowed allowed;
     if (allow_lds((const void *)k_keys_wide<T, D, NW>, (int)lds, allowed)) return -1;
-    hipLaunchKernelGGL((k_keys_wide<T, D, NW>), dim3((unsigned)grid), dim3(64 * NW * WideTile<D>::DS), lds, st, a, (int)tiles);
+    hipLaunchKernelGGL((k_keys_wide<T, D, NW>), dim3((unsigned)((total + 63) / 64 * 64)), dim3(64 * NW * WideTile<D>::DS), lds, st, a, (int)tiles,
+                       (int)total);
     return check_hip(hipGetLastError(), "attention launch");
 }
 
@@ -871,7 +924,7 @@ template <class T, int D>
 static int launch_rows(hipStream_t st, KeysArgs a, const RowsPlan &p, int B) {
     a.parts = p.parts;
     const int64_t grid = p.tiles * p.parts;
-    if (grid * a.KV * (p.nw ? B : 1) > 0x7fffffff) {
+    if (grid * a.KV * (p.nw ? B : 1) > 0x7fffff00) {
         set_error("attention over keys: too many rows for a launch");
         return -1;
     }
