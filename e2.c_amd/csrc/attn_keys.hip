@@ -80,12 +80,13 @@ __device__ inline typename Half8<T>::type load8(const uint16_t *p) {
 __device__ inline int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
 
 // The blocks of a selection list that hold keys this tile may see, compacted in list order into LDS; returns
-// their number (every thread of the workgroup). blocks: those below it may be read.
-__device__ inline int read_list(const int32_t *sel, int n_sel, int blocks, int *list, int *count) {
+// their number (every thread of the workgroup). first: this lane's of its first 64 entries; blocks: those below it may be
+// read.
+__device__ inline int read_list(const int32_t *sel, int n_sel, int first, int blocks, int *list, int *count) {
     if (threadIdx.x < 64) {
         int n = 0;
         for (int i = 0; i < n_sel; i += 64) {
-            const int e = i + (int)threadIdx.x < n_sel ? sel[i + threadIdx.x] : -1;
+            const int e = i == 0 ? first : i + (int)threadIdx.x < n_sel ? sel[i + threadIdx.x] : -1;
             const bool keep = e >= 0 && e < blocks;
             const uint64_t mask = __ballot(keep);
             if (keep) list[n + __popcll(mask & ((1ull << threadIdx.x) - 1))] = e;
@@ -112,6 +113,12 @@ template <int R>
 __device__ inline bool start_walk(const KeysArgs &a, int kvh, int b, int tile, int part, int *list, int *count, Walk &w) {
     const int G = a.G;
     w.kvh = kvh, w.b = b, w.part = part;
+    const int32_t *sel = nullptr;
+    int first = -1;  // requested before the ranges, whose latency it would otherwise follow
+    if (a.mode == kSelected) {
+        sel = a.sel + (((int64_t)b * a.NQ + tile / ((a.q_block * G + R - 1) / R)) * a.KV + kvh) * a.n_sel;
+        if ((int)threadIdx.x < min(a.n_sel, 64)) first = sel[threadIdx.x];
+    }
     w.qs = 0, w.nq = a.Mq, w.ks = 0, w.nk = 0;
     if (a.mode != kAllRows) {
         if (!row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, w.qs, w.nq)) return false;
@@ -133,8 +140,7 @@ __device__ inline bool start_walk(const KeysArgs &a, int kvh, int b, int tile, i
     int n_own = 0;
     w.n_pre = 0;
     if (a.mode == kSelected) {
-        const int32_t *sel = a.sel + (((int64_t)b * a.NQ + w.tok0 / a.q_block) * a.KV + kvh) * a.n_sel;
-        n_own = 2 * read_list(sel, a.n_sel, far > 0 ? (far + kKeyBlock - 1) / kKeyBlock : 0, list, count);
+        n_own = 2 * read_list(sel, a.n_sel, first, far > 0 ? (far + kKeyBlock - 1) / kKeyBlock : 0, list, count);
     } else {
         w.n_pre = (a.pre.rows + 31) / 32;
         if (a.mode == kOwnRows && far > 0) n_own = (far + 31) / 32;
@@ -178,7 +184,7 @@ __device__ inline void write_share(const KeysArgs &a, int64_t row, float mx, flo
     *(float2 *)(a.part_ml + row * 2) = make_float2(sum == sum ? mx : INFINITY, sum);
 }
 
-// Few rows: 16 a workgroup, whose waves take every WV-th key tile of 32 and are joined through LDS. Bound by HBM, hence by
+// Few rows: 16 RT a workgroup, whose waves take every WV-th key tile of 32 and are joined through LDS. Bound by HBM, hence by
 // what is in flight: each wave has LDS for a K and a V^T tile of its own and requests the next K tile when its logits are
 // done, the next V^T tile when its context is (direct-to-LDS loads, no barrier: 128 KB in flight a CU at head_dim 256).
 // Fragments loaded from global memory straight into registers took four times as long: neighbouring lanes of an operand
@@ -186,6 +192,7 @@ __device__ inline void write_share(const KeysArgs &a, int64_t row, float mx, flo
 //
 // 16x16x32 MFMA. Logits of 32 keys are two products whose K rows are permuted (row 4 x + i of product u holds key
 // 8 x + 4 u + i), so that a lane ends with 8 consecutive keys of one row, the operand of the next product.
+// RT 2: two tiles of 16 rows share the fragments, where a tile of 16 would read the keys twice.
 // LDS: K row i (2 D bytes) holds key i, its 16-byte chunk x at position x ^ f(i); V^T row d (64 bytes) its chunk x at
 // x ^ ((d >> 2) & 3): 16 lanes of a read hit 16 bank groups.
 typedef float f4v __attribute__((ext_vector_type(4)));
@@ -194,12 +201,13 @@ __device__ inline f4v mma16(typename Half8<T>::type a, typename Half8<T>::type b
     if constexpr (__is_same(T, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-template <int D>
+template <int D, int RT>
 struct FewTile {
     static constexpr int WV = D == 512 ? 2 : 4;              // waves
     static constexpr int kTile = 64 * D, kWave = 2 * kTile;  // bytes of a K (or V^T) tile; of a wave
     static constexpr int PITCH = D + 4;                      // floats of a row when the waves are joined
-    static constexpr int kBytes = WV * kWave > WV * 16 * PITCH * 4 ? WV * kWave : WV * 16 * PITCH * 4;
+    static constexpr int ROWS = 16 * RT;
+    static constexpr int kBytes = WV * kWave > WV * ROWS * PITCH * 4 ? WV * kWave : WV * ROWS * PITCH * 4;
 };
 // dma16 without a compiler memory clobber: the kernels order these loads with their reads by explicit waits
 __device__ inline void dma16_nc(v4u r, uint32_t lds, uint32_t voff, uint32_t soff) {
@@ -215,21 +223,21 @@ __device__ inline uint32_t here(uint32_t x) {
     return x;
 }
 
-template <class T, int D>
-__global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
+template <class T, int D, int RT>
+__global__ __launch_bounds__((64 * FewTile<D, RT>::WV)) void k_keys_few(KeysArgs a) {
     typedef typename Half8<T>::type V8;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    using L = FewTile<D>;
-    constexpr int WV = L::WV, NQ = D / 32, NO = D / 16, PITCH = L::PITCH;
+    using L = FewTile<D, RT>;
+    constexpr int WV = L::WV, ROWS = L::ROWS, NQ = D / 32, NO = D / 16, PITCH = L::PITCH;
     constexpr int RPI = 512 / D, LPR = D / 8, NL = D / 16;  // K rows a load fetches, lanes per K row, loads of a tile
     extern __shared__ __align__(16) unsigned char few_smem[];  // the waves' tiles, then the list (kSelected)
-    __shared__ float s_m[WV][16], s_l[WV][16];
+    __shared__ float s_m[WV][ROWS], s_l[WV][ROWS];
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int *list = (int *)(few_smem + L::kBytes);
     Walk k;
-    if (!start_walk<16>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
+    if (!start_walk<ROWS>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
                         &s_count, k))
         return;
     unsigned char *sk = few_smem + w * L::kWave, *sv = sk + L::kTile;
@@ -264,19 +272,24 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
         load_k(now);
         load_v(now);
     }
-    int last;  // own keys this lane's row sees
-    V8 qf[NQ];
-    {
-        const int r = min(k.r0 + c, k.rows - 1), tok = k.tok0 + r / a.G, h = k.kvh * a.G + r % a.G;
-        last = a.causal ? min(tok + k.back, k.nk - 1) : k.nk - 1;
+    int last[RT];  // own keys this lane's rows see
+    V8 qf[RT][NQ];
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        const int r = min(k.r0 + 16 * x + c, k.rows - 1), tok = k.tok0 + r / a.G, h = k.kvh * a.G + r % a.G;
+        last[x] = a.causal ? min(tok + k.back, k.nk - 1) : k.nk - 1;
         const uint16_t *qp = a.q + ((int64_t)k.qs + tok) * a.ldq + (int64_t)h * D + 8 * g;
 #pragma unroll
-        for (int s = 0; s < NQ; s++) qf[s] = *(const V8 *)(qp + 32 * s);
+        for (int s = 0; s < NQ; s++) qf[x][s] = *(const V8 *)(qp + 32 * s);
     }
-    f4v o[NO];
+    f4v o[RT][NO];
+    float mrun[RT], lrun[RT];
 #pragma unroll
-    for (int i = 0; i < NO; i++) o[i] = (f4v){};
-    float mrun = -INFINITY, lrun = 0.f;
+    for (int x = 0; x < RT; x++) {
+        mrun[x] = -INFINITY, lrun[x] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NO; i++) o[x][i] = (f4v){};
+    }
     uint32_t krd[2];
     const int fc = f_of(8 * (c >> 2) + (c & 3));  // the same for both products' rows
 #pragma unroll
@@ -288,47 +301,53 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
         const bool more = t + WV < k.t1;
         // the tile's K has landed (V^T was requested after it)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
-        f4v st[2] = {};
+        f4v st[RT][2] = {};
 #pragma unroll
         for (int s = 0; s < NQ; s++)
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-                st[u] = mma16<T>(*(const V8 *)(sk + krd[u] + (((4 * s + g) ^ fc) << 4)), qf[s], st[u]);
+            for (int u = 0; u < 2; u++) {
+                const V8 kf = *(const V8 *)(sk + krd[u] + (((4 * s + g) ^ fc) << 4));
+#pragma unroll
+                for (int x = 0; x < RT; x++) st[x][u] = mma16<T>(kf, qf[x][s], st[x][u]);
+            }
         if (more) {
             next = key_tile(a, k, list, t + WV);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its reads are done
             load_k(next);
         }
-        float tv[8];
+        V8 pb[RT];
 #pragma unroll
-        for (int i = 0; i < 8; i++) tv[i] = st[i >> 2][i & 3];
-        if (now.n < 32 || (!now.pre && a.causal)) {
-            const int top = now.pre ? now.n - 1 : min(last - now.key0, now.n - 1);
+        for (int x = 0; x < RT; x++) {
+            float tv[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (8 * g + i > top) tv[i] = -INFINITY;
-        }
-        float mloc = tv[0];
+            for (int i = 0; i < 8; i++) tv[i] = st[x][i >> 2][i & 3];
+            if (now.n < 32 || (!now.pre && a.causal)) {
+                const int top = now.pre ? now.n - 1 : min(last[x] - now.key0, now.n - 1);
 #pragma unroll
-        for (int i = 1; i < 8; i++) mloc = fmaxf(mloc, tv[i]);
-        mloc = fmaxf(mloc, xor_lane<16>(mloc));
-        mloc = fmaxf(mloc, xor_lane<32>(mloc));
-        const float mc = mloc * a.c2;
-        const bool moved = mc > mrun + kTau;
-        if (__any(moved)) {
-            const float alpha = moved ? __builtin_amdgcn_exp2f(mrun - mc) : 1.f;
-            mrun = moved ? mc : mrun;
-            lrun *= alpha;
+                for (int i = 0; i < 8; i++)
+                    if (8 * g + i > top) tv[i] = -INFINITY;
+            }
+            float mloc = tv[0];
 #pragma unroll
-            for (int i = 0; i < NO; i++) o[i] *= alpha;
-        }
-        const float ms = mrun == -INFINITY ? 0.f : mrun;
-        V8 pb;
+            for (int i = 1; i < 8; i++) mloc = fmaxf(mloc, tv[i]);
+            mloc = fmaxf(mloc, xor_lane<16>(mloc));
+            mloc = fmaxf(mloc, xor_lane<32>(mloc));
+            const float mc = mloc * a.c2;
+            const bool moved = mc > mrun[x] + kTau;
+            if (__any(moved)) {
+                const float alpha = moved ? __builtin_amdgcn_exp2f(mrun[x] - mc) : 1.f;
+                mrun[x] = moved ? mc : mrun[x];
+                lrun[x] *= alpha;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(tv[i], a.c2, -ms));
-            lrun += p;
-            pb[i] = (T)p;
+                for (int i = 0; i < NO; i++) o[x][i] *= alpha;
+            }
+            const float ms = mrun[x] == -INFINITY ? 0.f : mrun[x];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(tv[i], a.c2, -ms));
+                lrun[x] += p;
+                pb[x][i] = (T)p;
+            }
         }
         // the tile's V^T has landed (the next K was requested after it)
         if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
@@ -342,7 +361,11 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < NO; i++) o[i] = mma16<T>(*(const V8 *)(sv + vrd + i * 1024), pb, o[i]);
+        for (int i = 0; i < NO; i++) {
+            const V8 vf = *(const V8 *)(sv + vrd + i * 1024);
+#pragma unroll
+            for (int x = 0; x < RT; x++) o[x][i] = mma16<T>(vf, pb[x], o[x][i]);
+        }
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             load_v(next);
@@ -350,19 +373,23 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
     }
 
     // join the waves: contexts as they are, with their maxima and sums; a quad of dims a thread
-    float lsum = lrun + xor_lane<16>(lrun);
-    lsum += xor_lane<32>(lsum);
-    if (g == 0) s_m[w][c] = mrun, s_l[w][c] = lsum;
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        float lsum = lrun[x] + xor_lane<16>(lrun[x]);
+        lsum += xor_lane<32>(lsum);
+        if (g == 0) s_m[w][16 * x + c] = mrun[x], s_l[w][16 * x + c] = lsum;
+    }
     __syncthreads();  // the tiles are read
     float *ctx = (float *)few_smem;
-    {
-        float *y = ctx + (w * 16 + c) * PITCH + 4 * g;
 #pragma unroll
-        for (int i = 0; i < NO; i++) *(f4v *)(y + 16 * i) = o[i];
+    for (int x = 0; x < RT; x++) {
+        float *y = ctx + (w * ROWS + 16 * x + c) * PITCH + 4 * g;
+#pragma unroll
+        for (int i = 0; i < NO; i++) *(f4v *)(y + 16 * i) = o[x][i];
     }
     __syncthreads();
 #pragma unroll 1
-    for (int at = tid; at < 4 * D; at += 64 * WV) {
+    for (int at = tid; at < ROWS * D / 4; at += 64 * WV) {
         const int row = at / (D / 4), d = at % (D / 4) * 4, r = k.r0 + row;
         float mall = s_m[0][row];
 #pragma unroll
@@ -372,7 +399,7 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
 #pragma unroll
         for (int x = 0; x < WV; x++) {
             const float mx = s_m[x][row], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mall);
-            v += *(const f4v *)(ctx + (x * 16 + row) * PITCH + d) * f;
+            v += *(const f4v *)(ctx + (x * ROWS + row) * PITCH + d) * f;
             sum += s_l[x][row] * f;
         }
         if (sum != sum) v = (f4v)NAN;
@@ -843,7 +870,7 @@ __global__ __launch_bounds__(256) void k_keys_merge(KeysArgs a) {
 
 // ---- host: plan, checks, launches
 
-// How a set of rows runs: nw = 0: k_keys_few, else k_keys_wide with nw waves.
+// How a set of rows runs: k_keys_few with tiles of 16 (nw 0) or 32 rows (nw 1), else k_keys_wide with nw row groups of 32.
 struct RowsPlan {
     int nw = 0, parts = 1;
     int64_t tiles = 0;  // per sequence and kv head
@@ -868,13 +895,15 @@ static int key_shares(int64_t groups, int64_t tiles, int per, int least, int mos
 // groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles
 static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int most) {
     RowsPlan p;
-    p.nw = rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
-    // one launch of few rows that cannot fill the device even in shares: half as many rows a workgroup
-    if (p.nw == 4 && (rows + 127) / 128 * count * most < num_cus()) p.nw = 2;
+    p.nw = rows <= 16 ? 0 : rows <= 32 ? (D < 512 ? 1 : 0) : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
+    // Rows that cannot fill the device in tiles of 128 even in shares: tiles of 32 with 128 KB of keys in flight a CU beat
+    // them by reading the keys several times (from L2). 64 streams of 4 heads on 2 kv heads behind 16384 keys, head_dim
+    // 256, us of the prefix's launch: XX | YY.
+    if (p.nw >= 2 && D < 512 && (rows + 127) / 128 * count * 32 < num_cus()) p.nw = 1;
     const int R = p.nw ? 32 * p.nw : 16;
     p.tiles = (rows + R - 1) / R;
     // k_keys_few fills a CU's LDS from head_dim 256 on
-    p.parts = key_shares(p.tiles * count, tiles, p.nw || D < 256 ? 2 : 1, p.nw ? 8 : 4, most);
+    p.parts = key_shares(p.tiles * count, tiles, p.nw >= 2 || D < 256 ? 2 : 1, p.nw >= 2 ? 8 : 4, most);
     return p;
 }
 
@@ -920,6 +949,15 @@ static int launch_wide(hipStream_t st, const KeysArgs &a, int64_t tiles, int64_t
     return check_hip(hipGetLastError(), "attention launch");
 }
 
+template <class T, int D, int RT>
+static int launch_few(hipStream_t st, const KeysArgs &a, int64_t grid, int B) {
+    const size_t lds = FewTile<D, RT>::kBytes + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
+    static LdsAllowed allowed;
+    if (allow_lds((const void *)k_keys_few<T, D, RT>, (int)lds, allowed)) return -1;
+    hipLaunchKernelGGL((k_keys_few<T, D, RT>), dim3((unsigned)grid, a.KV, B), dim3(64 * FewTile<D, RT>::WV), lds, st, a);
+    return check_hip(hipGetLastError(), "attention launch");
+}
+
 template <class T, int D>
 static int launch_rows(hipStream_t st, KeysArgs a, const RowsPlan &p, int B) {
     a.parts = p.parts;
@@ -931,13 +969,10 @@ static int launch_rows(hipStream_t st, KeysArgs a, const RowsPlan &p, int B) {
     if (p.nw == 2) return launch_wide<T, D, 2>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 3) return launch_wide<T, D, 3>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 4) return launch_wide<T, D, 4>(st, a, p.tiles, grid * a.KV * B);
-    const size_t lds = FewTile<D>::kBytes + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
-    static LdsAllowed allowed;
-    if (allow_lds((const void *)k_keys_few<T, D>, (int)lds, allowed)) return -1;
-    hipLaunchKernelGGL((k_keys_few<T, D>), dim3((unsigned)grid, a.KV, B), dim3(64 * FewTile<D>::WV), lds, st, a);
-    return check_hip(hipGetLastError(), "attention launch");
+    // head_dim 512 has no registers for two tiles of rows
+    if (D < 512 && p.nw == 1) return launch_few<T, D, D < 512 ? 2 : 1>(st, a, grid, B);
+    return launch_few<T, D, 1>(st, a, grid, B);
 }
-
 // a copy of a set's V^T in rows of 16-byte multiples at `to` (columns past its rows: zeros)
 static int pad_values(hipStream_t st, KeySet &s, int KV, int D, uint16_t *to) {
     const int64_t ld = ((int64_t)s.rows + 7) / 8 * 8;
