@@ -440,18 +440,16 @@ __global__ __launch_bounds__((64 * FewTile<D, RT>::WV)) void k_keys_few(KeysArgs
 // chunk x sits at position x ^ (i & 7); chunk c of V^T row d at position c ^ ((d >> 2) & 3): the eight lanes of a
 // read group hit eight bank groups. Two buffers of both; at DS = 2 K has one, which the barrier of the logits'
 // exchange frees, and the exchange takes its place.
-template <int D>
+template <int D, int NW>
 struct WideTile {
     static constexpr int DS = D == 512 ? 2 : 1;     // waves that share a row group's dims
     static constexpr int kTile = 64 * D;            // bytes of a K or V^T tile
-    static constexpr int KB = DS == 1 ? 2 : 1;      // K buffers
+    static constexpr int KB = DS == 2 || (D <= 128 && NW == 2) ? 1 : 2;  // K buffers
     static constexpr int kV = KB * kTile;           // V^T's two
     static constexpr int kX = kV + 2 * kTile;       // the exchange: 4 KB a wave
     static constexpr int PITCH = 68;                // floats of a row of 64 dims on its way out
-    static constexpr int bytes(int nw) {
-        const int walk = kX + (DS > 1 ? nw * DS * 4096 : 0), out = nw * DS * 32 * PITCH * 4;
-        return walk > out ? walk : out;
-    }
+    static constexpr int kWalk = kX + (DS > 1 ? NW * DS * 4096 : 0), kOut = NW * DS * 32 * PITCH * 4;
+    static constexpr int kBytes = kWalk > kOut ? kWalk : kOut;
 };
 // The work of a workgroup of a grid that is a multiple of 64. Runs of 8 consecutive tiles of a sequence, which read the same
 // keys, go to one XCD and its L2 (workgroup i runs on XCD i % 8); the runs are dealt out in turn, their order turned
@@ -463,10 +461,11 @@ __device__ inline int spread(int i) {
 }
 // Work item `item` of those that have rows, over sequences, kv heads and tiles of R rows in that order (a wave's lanes add up
 // 64 sequences at a time): with a grid of max_q rows a sequence, the tiles past short sequences' ends would leave
-// their XCDs idle. False past the last item.
+// their XCDs idle. Returns -1, past the last item their number.
 constexpr int kFindMost = 512;  // sequences; beyond, the sums take longer than idle workgroups
-__device__ inline bool find_tile(const KeysArgs &a, int R, int item, int &b, int &kvh, int &tile) {
+__device__ inline int find_tile(const KeysArgs &a, int R, int item, int &b, int &kvh, int &tile) {
     const int lane = threadIdx.x & 63;
+    const int asked = item;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         int s, nq, n = 0;
         if (b0 + lane < a.B && row_range(a.q_start, a.q_len, b0 + lane, a.max_q, a.Mq, s, nq))
@@ -483,19 +482,19 @@ __device__ inline bool find_tile(const KeysArgs &a, int R, int item, int &b, int
             const int l = __builtin_ctzll(__ballot(sum > item));
             const int mine = __builtin_amdgcn_readlane(n, l), at = item - (__builtin_amdgcn_readlane(sum, l) - mine), per = mine / a.KV;
             b = b0 + l, kvh = at / per, tile = at % per;
-            return true;
+            return -1;
         }
         item -= all;
     }
-    return false;
+    return asked - item;
 }
 // K and V^T fragments are read this many MFMAs ahead of their use
 constexpr int kAhead = 3;
 
 template <class T, int D, int NW>
-__global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(KeysArgs a, int tiles, int total) {
+__global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wide(KeysArgs a, int tiles, int total) {
     typedef typename Half8<T>::type V8;
-    using L = WideTile<D>;
+    using L = WideTile<D, NW>;
     constexpr int DS = L::DS, WV = NW * DS, DW = D / DS;  // waves, dims of a wave
     constexpr int NQ = DW / 16, NO = DW / 32;
     constexpr int RPI = 512 / D, LPR = D / 8;             // K rows a load fetches, lanes per K row
@@ -505,14 +504,23 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wu = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wu / DS, dim0 = wu % DS * DW;
-    int *list = (int *)(wide_smem + L::bytes(NW));
-    int id = spread(blockIdx.x);
-    if (id >= total) return;
-    const int part = id % a.parts;
+    int *list = (int *)(wide_smem + L::kBytes);
+    int id, part, b, kvh, tile;
+    if (a.mode == kSelected) {
+        // selected blocks lie near each other for neighbouring query blocks: one range of the tiles that have rows an XCD
+        int live = total / a.parts;
+        if (a.B > 1 && a.B <= kFindMost) live = find_tile(a, 32 * NW, 0x7fffffff, b, kvh, tile);
+        const int each = (live * a.parts + 7) / 8;
+        id = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+        if ((int)(blockIdx.x >> 3) >= each || id >= live * a.parts) return;
+    } else {
+        id = spread(blockIdx.x);
+        if (id >= total) return;
+    }
+    part = id % a.parts;
     id /= a.parts;
-    int b, kvh, tile;
     if (a.B > 1 && a.B <= kFindMost && a.mode != kAllRows) {
-        if (!find_tile(a, 32 * NW, id, b, kvh, tile)) return;
+        if (find_tile(a, 32 * NW, id, b, kvh, tile) >= 0) return;
     } else {
         tile = id % tiles;
         id /= tiles;
@@ -607,7 +615,7 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
     // the tile loads in flight
     __builtin_amdgcn_s_waitcnt(0x0F70);
     for (int t = k.t0; t < k.t1; t++, now = next) {
-        const int buf = (t - k.t0) & 1, kbuf = DS == 1 ? buf : 0;
+        const int buf = (t - k.t0) & 1, kbuf = L::KB == 2 ? buf : 0;
         // this wave's loads of tile t have landed; the barrier makes every wave's visible and ends every wave's
         // reads of the buffer that the next loads refill
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -627,7 +635,7 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
         }
         const bool work = active && now.n > 0;
         f16v st = (f16v){};
-        constexpr int NF = DS == 1 ? 2 * NLW : NLW;  // loads requested here: V^T's, then K's
+        constexpr int NF = L::KB == 2 ? 2 * NLW : NLW;  // loads requested here: V^T's, then K's
         auto request = [&](int j) {
             if (j < NLW) load_v(f, buf ^ 1, j);
             else load_k(f, buf ^ 1, j - NLW);
@@ -662,6 +670,11 @@ __global__ __launch_bounds__(64 * NW * WideTile<D>::DS, 2) void k_keys_wide(Keys
                 const float4 v = y[64 * i];
                 st[4 * i] += v.x, st[4 * i + 1] += v.y, st[4 * i + 2] += v.z, st[4 * i + 3] += v.w;
             }
+        }
+        if constexpr (L::KB == 1 && DS == 1) {
+            lds_barrier();  // as above
+#pragma unroll
+            for (int j = 0; j < NLW; j++) load_k(f, 0, j);
         }
         if (!work) continue;
         float tv[16];
@@ -941,10 +954,10 @@ static size_t workspace_of(const KeysPlan &p, int Mq, int H, int D) { return par
 
 template <class T, int D, int NW>
 static int launch_wide(hipStream_t st, const KeysArgs &a, int64_t tiles, int64_t total) {
-    const size_t lds = WideTile<D>::bytes(NW) + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
+    const size_t lds = WideTile<D, NW>::kBytes + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
     static LdsAllowed allowed;
     if (allow_lds((const void *)k_keys_wide<T, D, NW>, (int)lds, allowed)) return -1;
-    hipLaunchKernelGGL((k_keys_wide<T, D, NW>), dim3((unsigned)((total + 63) / 64 * 64)), dim3(64 * NW * WideTile<D>::DS), lds, st, a, (int)tiles,
+    hipLaunchKernelGGL((k_keys_wide<T, D, NW>), dim3((unsigned)((total + 63) / 64 * 64)), dim3((64 * NW * WideTile<D, NW>::DS)), lds, st, a, (int)tiles,
                        (int)total);
     return check_hip(hipGetLastError(), "attention launch");
 }
