@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "attn_keys.h"
 
@@ -212,6 +213,12 @@ struct FewTile {
 // dma16 without a compiler memory clobber: the kernels order these loads with their reads by explicit waits
 __device__ inline void dma16_nc(v4u r, uint32_t lds, uint32_t voff, uint32_t soff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff));
+}
+// The same with the LDS address as a base and an offset.
+template <int OFF>
+__device__ inline void dma16_at(v4u r, uint32_t lds, uint32_t voff, uint32_t soff) {
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds" ::"s"(lds), "n"(OFF), "v"(voff), "s"(r), "s"(soff)
+                 : "scc");
 }
 // x, not to be computed ahead for every load of a tile: that many scalars do not fit
 __device__ inline uint64_t here(uint64_t x) {
@@ -554,8 +561,10 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_void *)wide_smem);
     const int lr = lane / LPR, lc = lane % LPR;
     const int vchunk = (lane & 3) ^ ((lane >> 4) & 3);
-    // A tile's loads: load j of a wave takes K rows RPI x .. + RPI - 1 or V^T rows 16 x .. + 15, x = NLW wave + j.
-    // Descriptors start at the tile's first key, so 32 bits hold every offset at any length of the cache.
+    // A tile's loads: load j of a wave takes K rows RPI x .. + RPI - 1 or V^T rows 16 x .. + 15, x = NLW wave + j. A tile is
+    // about as many instructions as its MFMAs take cycles / 4, so what does not change from tile to tile is kept. Descriptors
+    // start at the tile's first key (V^T: and the wave's first row), so 32 bits hold every offset at any length of the
+    // cache; V^T's pitch is limited (wide_takes).
     struct Range {
         uint64_t k, v;      // addresses of its first key in this kv head; V^T: this wave's first row
         uint32_t ldk, ldv;  // bytes
@@ -567,35 +576,48 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
         r.ldk = (uint32_t)s.ldk * 2, r.ldv = (uint32_t)s.ldv * 2;
         return r;
     };
-    const Range own = range_of(a.own, k.ks), pre = range_of(a.pre, 0);
-    struct Fetch {
-        uint64_t k, v;
-        uint32_t ldk, ldv, bytes;  // K's range
-        uint32_t ko, vo;           // lane offsets
+    const Range own = range_of(a.own, k.ks);
+    v4u rv, rk;
+    uint32_t krow[NLW], vrow, ldk, klane, vlane, vo;  // offsets of K's rows, of 16 rows of V^T; of lanes; the tile's of V^T
+    uint64_t kbase, vbase;
+    auto enter = [&](const Range &r) {
+#pragma unroll
+        for (int j = 0; j < NLW; j++) krow[j] = __builtin_amdgcn_readfirstlane((uint32_t)swap23(RPI * (NLW * wu + j)) * r.ldk);
+        kbase = r.k, ldk = r.ldk, vbase = r.v, vrow = 16 * r.ldv;
+        klane = (uint32_t)swap23(lr) * r.ldk;
+        vlane = (uint32_t)(lane >> 2) * r.ldv + (uint32_t)vchunk * 16;
     };
-    auto fetch_of = [&](const KeyTile &kt) {
-        Fetch f;
-        f.ldk = kt.pre ? pre.ldk : own.ldk, f.ldv = kt.pre ? pre.ldv : own.ldv;
-        f.k = (kt.pre ? pre.k : own.k) + (uint64_t)(uint32_t)kt.key0 * f.ldk;
-        f.v = (kt.pre ? pre.v : own.v) + 2 * (uint64_t)(uint32_t)kt.key0;
-        f.bytes = kt.n ? (uint32_t)(kt.n - 1) * f.ldk + 2 * D : 0;
-        f.ko = (uint32_t)swap23(lr) * f.ldk;
-        f.vo = 8 * vchunk < kt.n ? (uint32_t)(lane >> 2) * f.ldv + (uint32_t)vchunk * 16 : 0x80000000u;
-        return f;
+    auto fetch = [&](const KeyTile &kt) {
+        rk = rsrc_words((const void *)(kbase + (uint64_t)(uint32_t)kt.key0 * ldk), kt.n ? (uint32_t)(kt.n - 1) * ldk + 2 * D : 0);
+        rv = rsrc_words((const void *)(vbase + 2 * (uint64_t)(uint32_t)kt.key0), 0x7fffffffu);
+        vo = 8 * vchunk < kt.n ? vlane : 0x80000000u;
     };
     const uint32_t kchunk = (uint32_t)((lc ^ (lr & 7)) << 4);
-    auto load_k = [&](const Fetch &f, int buf, int j) {
+    const uint32_t ldsw = lds0 + (uint32_t)(NLW * wu * 1024);
+    auto load_k = [&](int buf, auto jj) {
+        constexpr int j = decltype(jj)::value;
         const int x = NLW * wu + j, i = RPI * x;
         if (NL % WV && x >= NL) return;
         // row i + lr: chunk lc ^ ((i + lr) & 7). A row past the range reads as zero: its offset lies past the descriptor's end
-        dma16_nc(rsrc_words((const void *)f.k, f.bytes), lds0 + (uint32_t)(buf * L::kTile + i * (2 * D)),
-                 f.ko + (kchunk ^ here((uint32_t)((i & 7) << 4))), here((uint32_t)swap23(i) * f.ldk));
+        dma16_at<j * 1024>(rk, ldsw + (uint32_t)(buf * L::kTile), klane + (kchunk ^ here((uint32_t)((i & 7) << 4))), krow[j]);
     };
-    auto load_v = [&](const Fetch &f, int buf, int j) {
+    auto load_v = [&](int buf, auto jj) {
+        constexpr int j = decltype(jj)::value;
         if (NL % WV && NLW * wu + j >= NL) return;
-        const v4u rs = rsrc_words((const void *)here(f.v + (uint64_t)(16 * j) * f.ldv), 0x7fffffffu);
-        dma16_nc(rs, lds0 + (uint32_t)(L::kV + buf * L::kTile + (NLW * wu + j) * 1024), f.vo, 0);
+        dma16_at<L::kV + j * 1024>(rv, ldsw + (uint32_t)(buf * L::kTile), vo, here(j * vrow));
     };
+    // requests `from` .. `to` - 1 of a tile: V^T's loads, then K's
+    auto request = [&]<int... J>(std::integer_sequence<int, J...>, int vbuf, int kbuf_, auto from, auto to) {
+        auto one = [&](auto jj) {
+            constexpr int j = decltype(jj)::value;
+            if constexpr (j >= decltype(from)::value && j < decltype(to)::value) {
+                if constexpr (j < NLW) load_v(vbuf, std::integral_constant<int, j>{});
+                else load_k(kbuf_, std::integral_constant<int, j - NLW>{});
+            }
+        };
+        (one(std::integral_constant<int, J>{}), ...);
+    };
+    constexpr auto kEach = std::make_integer_sequence<int, 2 * NLW>{};
 
     const int kkey = lane & 31;
     // fragment reads: K chunk 2 s + half of row kkey (s = 4 t + u: 128 t + ((2 u + half) ^ (kkey & 7)) * 16), V^T chunk
@@ -604,12 +626,11 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
     const uint32_t vrd = (uint32_t)(L::kV + (dim0 + kkey) * 64 + ((half ^ ((kkey >> 2) & 3)) << 4));
 
     KeyTile now = {}, next = {};
-    Fetch f = {};
     if (k.t0 < k.t1) {
         now = key_tile(a, k, list, k.t0);
-        f = fetch_of(now);
-#pragma unroll
-        for (int j = 0; j < NLW; j++) load_k(f, 0, j), load_v(f, 0, j);
+        enter(now.pre ? range_of(a.pre, 0) : own);
+        fetch(now);
+        request(kEach, 0, 0, std::integral_constant<int, 0>{}, std::integral_constant<int, 2 * NLW>{});
     }
     // the Q loads are waited for here, by a wait that the compiler's count sees: inside the loop it would cover
     // the tile loads in flight
@@ -622,7 +643,8 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
         __syncthreads();
         // the next tile; after the last one that again, which nobody reads, so that no branch parts the loads from the MFMAs
         next = key_tile(a, k, list, min(t + 1, k.t1 - 1));
-        f = fetch_of(next);
+        if (next.pre != now.pre) enter(own);
+        fetch(next);
         unsigned char *sk = wide_smem + kbuf * L::kTile, *sv = wide_smem + buf * L::kTile;
         if (now.n & 7) {  // values past the range in its last chunk (of any bits) become 0
             for (int d = tid; d < D; d += 64 * WV) {
@@ -636,34 +658,31 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
         const bool work = active && now.n > 0;
         f16v st = (f16v){};
         constexpr int NF = L::KB == 2 ? 2 * NLW : NLW;  // loads requested here: V^T's, then K's
-        auto request = [&](int j) {
-            if (j < NLW) load_v(f, buf ^ 1, j);
-            else load_k(f, buf ^ 1, j - NLW);
-        };
         if (work) {
             V8 kr[kAhead];
             auto kfrag = [&](int s) { return *(const V8 *)(sk + (krd ^ (uint32_t)((s & 3) << 5)) + (s >> 2) * 128); };
 #pragma unroll
             for (int s = 0; s < kAhead; s++) kr[s] = kfrag(s);
-#pragma unroll
-            for (int s = 0; s < NQ; s++) {
-                st = Half8<T>::mma(kr[s % kAhead], qf[s], st);
-                if (s + kAhead < NQ) kr[s % kAhead] = kfrag(s + kAhead);
-#pragma unroll
-                for (int j = s * NF / NQ; j < (s + 1) * NF / NQ; j++) request(j);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            [&]<int... S>(std::integer_sequence<int, S...>) {
+                auto one = [&](auto ss) {
+                    constexpr int s = decltype(ss)::value;
+                    st = Half8<T>::mma(kr[s % kAhead], qf[s], st);
+                    if constexpr (s + kAhead < NQ) kr[s % kAhead] = kfrag(s + kAhead);
+                    request(kEach, buf ^ 1, buf ^ 1, std::integral_constant<int, s * NF / NQ>{},
+                            std::integral_constant<int, (s + 1) * NF / NQ>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                (one(std::integral_constant<int, S>{}), ...);
+            }(std::make_integer_sequence<int, NQ>{});
         } else {
-#pragma unroll
-            for (int j = 0; j < NF; j++) request(j);
+            request(kEach, buf ^ 1, buf ^ 1, std::integral_constant<int, 0>{}, std::integral_constant<int, NF>{});
         }
         if constexpr (DS == 2) {
             float4 *x = (float4 *)(wide_smem + L::kX) + wu * 256 + lane;
 #pragma unroll
             for (int i = 0; i < 4; i++) x[64 * i] = make_float4(st[4 * i], st[4 * i + 1], st[4 * i + 2], st[4 * i + 3]);
             lds_barrier();  // the K tile is read: its buffer takes the next one
-#pragma unroll
-            for (int j = 0; j < NLW; j++) load_k(f, 0, j);
+            request(kEach, 0, 0, std::integral_constant<int, NLW>{}, std::integral_constant<int, 2 * NLW>{});
             const float4 *y = (const float4 *)(wide_smem + L::kX) + (wu ^ 1) * 256 + lane;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -673,8 +692,7 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
         }
         if constexpr (L::KB == 1 && DS == 1) {
             lds_barrier();  // as above
-#pragma unroll
-            for (int j = 0; j < NLW; j++) load_k(f, 0, j);
+            request(kEach, 0, 0, std::integral_constant<int, NLW>{}, std::integral_constant<int, 2 * NLW>{});
         }
         if (!work) continue;
         float tv[16];
@@ -905,13 +923,17 @@ static int key_shares(int64_t groups, int64_t tiles, int per, int least, int mos
     return n < 1 ? 1 : (int)n;
 }
 
+// k_keys_wide's offsets into V^T within a wave's rows (up to 128) are 32 bits: caches past 8 M columns take k_keys_few
+static bool wide_takes(const KeySet &s) { return !s.rows || s.ldv < (1 << 23); }
+
 // groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles
-static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int most) {
+static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int most, bool wide) {
     RowsPlan p;
     p.nw = rows <= 16 ? 0 : rows <= 32 ? (D < 512 ? 1 : 0) : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
     // Rows that cannot fill the device in tiles of 128 even in shares: tiles of 32 with 128 KB of keys in flight a CU beat
     // them by reading the keys several times (from L2). 64 streams of 4 heads on 2 kv heads behind 16384 keys, head_dim
     // 256, us of the prefix's launch: XX | YY.
+    if (!wide && p.nw >= 2) p.nw = D < 512 ? 1 : 0;
     if (p.nw >= 2 && D < 512 && (rows + 127) / 128 * count * 32 < num_cus()) p.nw = 1;
     const int R = p.nw ? 32 * p.nw : 16;
     p.tiles = (rows + R - 1) / R;
@@ -931,8 +953,9 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
     const int64_t rows = (int64_t)max_q * G;
     // sequences of less than a tile share the prefix's tiles
     p.apart = B > 1 && P > 0 && rows < 32;
-    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, D, kMaxKeyParts / 2);
-    p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), D, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts);
+    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, D, kMaxKeyParts / 2, wide_takes(pre));
+    p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), D, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts,
+                       wide_takes(own) && (p.apart || wide_takes(pre)));
     if (needs_copy(pre)) p.pad_pre = pad_bytes(P, KV, D);
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
@@ -941,7 +964,7 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
 static KeysPlan plan_blocks(const KeySet &own, int B, int max_q, int H, int KV, int D, int q_block, int n_sel) {
     KeysPlan p;
     const int64_t NQ = ((int64_t)max_q + q_block - 1) / q_block;
-    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, D, kMaxKeyParts);
+    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, D, kMaxKeyParts, wide_takes(own));
     p.rows.tiles *= NQ;
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
