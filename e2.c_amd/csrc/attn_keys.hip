@@ -466,35 +466,46 @@ __device__ inline int spread(int i) {
     const int xcd = i & 7, slot = i >> 3, round = slot >> 3;
     return (round * 8 + ((xcd + round + (round >> 2)) & 7)) * 8 + (slot & 7);
 }
-// Work item `item` of those that have rows, over sequences, kv heads and tiles of R rows in that order (a wave's lanes add up
-// 64 sequences at a time): with a grid of max_q rows a sequence, the tiles past short sequences' ends would leave
-// their XCDs idle. Returns -1, past the last item their number.
+// The work items that have rows, over sequences, kv heads and tiles of R rows in that order (a wave's lanes add up 64
+// sequences at a time): with a grid of max_q rows a sequence, the tiles past short sequences' ends would leave their
+// XCDs idle.
 constexpr int kFindMost = 512;  // sequences; beyond, the sums take longer than idle workgroups
-__device__ inline int find_tile(const KeysArgs &a, int R, int item, int &b, int &kvh, int &tile) {
-    const int lane = threadIdx.x & 63;
-    const int asked = item;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        int s, nq, n = 0;
-        if (b0 + lane < a.B && row_range(a.q_start, a.q_len, b0 + lane, a.max_q, a.Mq, s, nq))
-            n = a.mode == kSelected ? (nq + a.q_block - 1) / a.q_block * ((a.q_block * a.G + R - 1) / R) : (nq * a.G + R - 1) / R;
-        n *= a.KV;
-        int sum = n;
+struct LiveTiles {
+    int n, sum, all, at;  // of 64 sequences from `at` on: a lane's items, with those of the lanes before, all lanes'
+    __device__ inline void add(const KeysArgs &a, int R, int from) {
+        const int lane = threadIdx.x & 63;
+        int s, nq;
+        n = 0, at = from;
+        if (from + lane < a.B && row_range(a.q_start, a.q_len, from + lane, a.max_q, a.Mq, s, nq))
+            n = a.KV * (a.mode == kSelected ? (nq + a.q_block - 1) / a.q_block * ((a.q_block * a.G + R - 1) / R) : (nq * a.G + R - 1) / R);
+        sum = n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int v = __shfl_up(sum, o);
             if (lane >= o) sum += v;
         }
-        const int all = __builtin_amdgcn_readlane(sum, 63);
-        if (item < all) {
-            const int l = __builtin_ctzll(__ballot(sum > item));
-            const int mine = __builtin_amdgcn_readlane(n, l), at = item - (__builtin_amdgcn_readlane(sum, l) - mine), per = mine / a.KV;
-            b = b0 + l, kvh = at / per, tile = at % per;
-            return -1;
-        }
-        item -= all;
+        all = __builtin_amdgcn_readlane(sum, 63);
     }
-    return asked - item;
-}
+    __device__ inline int total(const KeysArgs &a, int R) {
+        int t = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) add(a, R, b0), t += all;
+        return t;
+    }
+    // the sequence, kv head and tile of an item; false past the last
+    __device__ inline bool find(const KeysArgs &a, int R, int item, int &b, int &kvh, int &tile) {
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
+            if (at != b0) add(a, R, b0);
+            if (item < all) {
+                const int l = __builtin_ctzll(__ballot(sum > item));
+                const int mine = __builtin_amdgcn_readlane(n, l), in = item - (__builtin_amdgcn_readlane(sum, l) - mine), per = mine / a.KV;
+                b = b0 + l, kvh = in / per, tile = in % per;
+                return true;
+            }
+            item -= all;
+        }
+        return false;
+    }
+};
 // K and V^T fragments are read this many MFMAs ahead of their use
 constexpr int kAhead = 3;
 
@@ -513,10 +524,12 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
     const int group = wu / DS, dim0 = wu % DS * DW;
     int *list = (int *)(wide_smem + L::kBytes);
     int id, part, b, kvh, tile;
+    const bool search = a.B > 1 && a.B <= kFindMost && a.mode != kAllRows;
+    LiveTiles lt;
+    lt.at = -1;
     if (a.mode == kSelected) {
         // selected blocks lie near each other for neighbouring query blocks: one range of the tiles that have rows an XCD
-        int live = total / a.parts;
-        if (a.B > 1 && a.B <= kFindMost) live = find_tile(a, 32 * NW, 0x7fffffff, b, kvh, tile);
+        const int live = search ? lt.total(a, 32 * NW) : total / a.parts;
         const int each = (live * a.parts + 7) / 8;
         id = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
         if ((int)(blockIdx.x >> 3) >= each || id >= live * a.parts) return;
@@ -526,8 +539,8 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
     }
     part = id % a.parts;
     id /= a.parts;
-    if (a.B > 1 && a.B <= kFindMost && a.mode != kAllRows) {
-        if (find_tile(a, 32 * NW, id, b, kvh, tile) >= 0) return;
+    if (search) {
+        if (!lt.find(a, 32 * NW, id, b, kvh, tile)) return;
     } else {
         tile = id % tiles;
         id /= tiles;

@@ -127,6 +127,7 @@ __device__ inline int byte_lanes_negative(uint32_t x) {  // 0xff in every negati
     const uint32_t m = (x >> 7) & 0x01010101u;
     return (int)((m << 8) - m);
 }
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int shares, int groups) {
     constexpr int NS = D / 32, TILE = 64 * D, RPI = 512 / D, LPR = D / 8, NLW = D / 64;
@@ -185,17 +186,17 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
             const bool row = live && in < R && tok < nq && in / a.G < a.q_block;
             const uint16_t *qp = a.q + (qs + (row ? tok : 0)) * a.ldq + (int64_t)(kvh * a.G + in % a.G) * D + 16 * half;
             uint32_t raw[NS][8];
-            float am = 0.f;
 #pragma unroll
             for (int s = 0; s < NS; s++) {
                 *(uint4 *)raw[s] = *(const uint4 *)(qp + 32 * s);
                 *(uint4 *)(raw[s] + 4) = *(const uint4 *)(qp + 32 * s + 8);
             }
+            us2 top = {0, 0};  // magnitudes order like the bits below the sign
 #pragma unroll
             for (int s = 0; s < NS; s++)
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    am = fmaxf(am, fmaxf(fabsf(value_of<T>((uint16_t)raw[s][e])), fabsf(value_of<T>((uint16_t)(raw[s][e] >> 16)))));
+                for (int e = 0; e < 8; e++) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, raw[s][e] & 0x7fff7fffu));
+            float am = value_of<T>(max(top[0], top[1]));
             am = fmaxf(am, xor_lane<32>(am));
             const QScale q = qscale(am);
 #pragma unroll
