@@ -940,7 +940,7 @@ static int key_shares(int64_t groups, int64_t tiles, int per, int least, int mos
 static bool wide_takes(const KeySet &s) { return !s.rows || s.ldv < (1 << 23); }
 
 // groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles
-static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int most, bool wide) {
+static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int most, bool wide, bool joined) {
     RowsPlan p;
     p.nw = rows <= 16 ? 0 : rows <= 32 ? (D < 512 ? 1 : 0) : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
     // Rows that cannot fill the device in tiles of 128 even in shares: tiles of 32 with 128 KB of keys in flight a CU beat
@@ -952,6 +952,9 @@ static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int
     p.tiles = (rows + R - 1) / R;
     // k_keys_few fills a CU's LDS from head_dim 256 on
     p.parts = key_shares(p.tiles * count, tiles, p.nw >= 2 || D < 256 ? 2 : 1, p.nw >= 2 ? 8 : 4, most);
+    // up to six tiles a wave, one workgroup's walk is shorter than a second launch to join shares (one token of 3 heads over
+    // 531 keys of 256, us a call: 12.9 | 16.1 in four shares), unless there is one anyway (`joined`)
+    if (p.nw < 2 && tiles <= 24 && !joined) p.parts = 1;
     return p;
 }
 
@@ -966,9 +969,9 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
     const int64_t rows = (int64_t)max_q * G;
     // sequences of less than a tile share the prefix's tiles
     p.apart = B > 1 && P > 0 && rows < 32;
-    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, D, kMaxKeyParts / 2, wide_takes(pre));
+    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, D, kMaxKeyParts / 2, wide_takes(pre), true);
     p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), D, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts,
-                       wide_takes(own) && (p.apart || wide_takes(pre)));
+                       wide_takes(own) && (p.apart || wide_takes(pre)), p.apart);
     if (needs_copy(pre)) p.pad_pre = pad_bytes(P, KV, D);
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
@@ -977,7 +980,7 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
 static KeysPlan plan_blocks(const KeySet &own, int B, int max_q, int H, int KV, int D, int q_block, int n_sel) {
     KeysPlan p;
     const int64_t NQ = ((int64_t)max_q + q_block - 1) / q_block;
-    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, D, kMaxKeyParts, wide_takes(own));
+    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, D, kMaxKeyParts, wide_takes(own), false);
     p.rows.tiles *= NQ;
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;

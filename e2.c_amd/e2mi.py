@@ -837,13 +837,17 @@ def rope(q, k, pos, freqs, H, KV, layout="half", magnitude=1.0, inverse=False, q
         nq = H
         if q_out is None:
             q_out = _new(stream, q.new_empty, (M, width))
-        po, lo = _rows("rope", q_out, M, width, dtype, dev)
+            po, lo = q_out.data_ptr(), width
+        else:
+            po, lo = _rows("rope", q_out, M, width, dtype, dev)
     if k is not None:
         pk, lk = _rows("rope", k, M, KV * D, dtype, dev)
         nk = KV
         if k_out is None:
             k_out = _new(stream, k.new_empty, (M, KV * D))
-        pt, lt = _rows("rope", k_out, M, KV * D, dtype, dev)
+            pt, lt = k_out.data_ptr(), KV * D
+        else:
+            pt, lt = _rows("rope", k_out, M, KV * D, dtype, dev)
     if freqs.dtype is not torch.float64 or freqs.get_device() != dev or not freqs.is_contiguous():
         raise E2MIError(f"rope: needs contiguous float64 frequencies on device {dev}")
     check(load().e2mi_rope(_stream(stream), kind, _LAYOUTS[layout], 1 if inverse else 0, pq, lq, po, lo, nq, pk, lk, pt, lt, nk, M,
