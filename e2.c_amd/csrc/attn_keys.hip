@@ -17,6 +17,7 @@
 // 16-byte chunks of 8 keys.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -185,7 +186,7 @@ __device__ inline void write_share(const KeysArgs &a, int64_t row, float mx, flo
     *(float2 *)(a.part_ml + row * 2) = make_float2(sum == sum ? mx : INFINITY, sum);
 }
 
-// Few rows: 16 RT a workgroup, whose waves take every WV-th key tile of 32 and are joined through LDS. Bound by HBM, hence by
+// Few rows: 16 a workgroup, whose waves take every WV-th key tile of 32 and are joined through LDS. Bound by HBM, hence by
 // what is in flight: each wave has LDS for a K and a V^T tile of its own and requests the next K tile when its logits are
 // done, the next V^T tile when its context is (direct-to-LDS loads, no barrier: 128 KB in flight a CU at head_dim 256).
 // Fragments loaded from global memory straight into registers took four times as long: neighbouring lanes of an operand
@@ -193,7 +194,6 @@ __device__ inline void write_share(const KeysArgs &a, int64_t row, float mx, flo
 //
 // 16x16x32 MFMA. Logits of 32 keys are two products whose K rows are permuted (row 4 x + i of product u holds key
 // 8 x + 4 u + i), so that a lane ends with 8 consecutive keys of one row, the operand of the next product.
-// RT 2: two tiles of 16 rows share the fragments, where a tile of 16 would read the keys twice.
 // LDS: K row i (2 D bytes) holds key i, its 16-byte chunk x at position x ^ f(i); V^T row d (64 bytes) its chunk x at
 // x ^ ((d >> 2) & 3): 16 lanes of a read hit 16 bank groups.
 typedef float f4v __attribute__((ext_vector_type(4)));
@@ -202,13 +202,12 @@ __device__ inline f4v mma16(typename Half8<T>::type a, typename Half8<T>::type b
     if constexpr (__is_same(T, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-template <int D, int RT>
+template <int D>
 struct FewTile {
     static constexpr int WV = D == 512 ? 2 : 4;              // waves
     static constexpr int kTile = 64 * D, kWave = 2 * kTile;  // bytes of a K (or V^T) tile; of a wave
     static constexpr int PITCH = D + 4;                      // floats of a row when the waves are joined
-    static constexpr int ROWS = 16 * RT;
-    static constexpr int kBytes = WV * kWave > WV * ROWS * PITCH * 4 ? WV * kWave : WV * ROWS * PITCH * 4;
+    static constexpr int kBytes = WV * kWave > WV * 16 * PITCH * 4 ? WV * kWave : WV * 16 * PITCH * 4;
 };
 // dma16 without a compiler memory clobber: the kernels order these loads with their reads by explicit waits
 __device__ inline void dma16_nc(v4u r, uint32_t lds, uint32_t voff, uint32_t soff) {
@@ -230,21 +229,21 @@ __device__ inline uint32_t here(uint32_t x) {
     return x;
 }
 
-template <class T, int D, int RT>
-__global__ __launch_bounds__((64 * FewTile<D, RT>::WV)) void k_keys_few(KeysArgs a) {
+template <class T, int D>
+__global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
     typedef typename Half8<T>::type V8;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    using L = FewTile<D, RT>;
-    constexpr int WV = L::WV, ROWS = L::ROWS, NQ = D / 32, NO = D / 16, PITCH = L::PITCH;
+    using L = FewTile<D>;
+    constexpr int WV = L::WV, NQ = D / 32, NO = D / 16, PITCH = L::PITCH;
     constexpr int RPI = 512 / D, LPR = D / 8, NL = D / 16;  // K rows a load fetches, lanes per K row, loads of a tile
     extern __shared__ __align__(16) unsigned char few_smem[];  // the waves' tiles, then the list (kSelected)
-    __shared__ float s_m[WV][ROWS], s_l[WV][ROWS];
+    __shared__ float s_m[WV][16], s_l[WV][16];
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int *list = (int *)(few_smem + L::kBytes);
     Walk k;
-    if (!start_walk<ROWS>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
+    if (!start_walk<16>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
                         &s_count, k))
         return;
     unsigned char *sk = few_smem + w * L::kWave, *sv = sk + L::kTile;
@@ -279,24 +278,19 @@ __global__ __launch_bounds__((64 * FewTile<D, RT>::WV)) void k_keys_few(KeysArgs
         load_k(now);
         load_v(now);
     }
-    int last[RT];  // own keys this lane's rows see
-    V8 qf[RT][NQ];
-#pragma unroll
-    for (int x = 0; x < RT; x++) {
-        const int r = min(k.r0 + 16 * x + c, k.rows - 1), tok = k.tok0 + r / a.G, h = k.kvh * a.G + r % a.G;
-        last[x] = a.causal ? min(tok + k.back, k.nk - 1) : k.nk - 1;
+    int last;  // own keys this lane's row sees
+    V8 qf[NQ];
+    {
+        const int r = min(k.r0 + c, k.rows - 1), tok = k.tok0 + r / a.G, h = k.kvh * a.G + r % a.G;
+        last = a.causal ? min(tok + k.back, k.nk - 1) : k.nk - 1;
         const uint16_t *qp = a.q + ((int64_t)k.qs + tok) * a.ldq + (int64_t)h * D + 8 * g;
 #pragma unroll
-        for (int s = 0; s < NQ; s++) qf[x][s] = *(const V8 *)(qp + 32 * s);
+        for (int s = 0; s < NQ; s++) qf[s] = *(const V8 *)(qp + 32 * s);
     }
-    f4v o[RT][NO];
-    float mrun[RT], lrun[RT];
+    f4v o[NO];
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        mrun[x] = -INFINITY, lrun[x] = 0.f;
-#pragma unroll
-        for (int i = 0; i < NO; i++) o[x][i] = (f4v){};
-    }
+    for (int i = 0; i < NO; i++) o[i] = (f4v){};
+    float mrun = -INFINITY, lrun = 0.f;
     uint32_t krd[2];
     const int fc = f_of(8 * (c >> 2) + (c & 3));  // the same for both products' rows
 #pragma unroll
@@ -308,53 +302,47 @@ __global__ __launch_bounds__((64 * FewTile<D, RT>::WV)) void k_keys_few(KeysArgs
         const bool more = t + WV < k.t1;
         // the tile's K has landed (V^T was requested after it)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
-        f4v st[RT][2] = {};
+        f4v st[2] = {};
 #pragma unroll
         for (int s = 0; s < NQ; s++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const V8 kf = *(const V8 *)(sk + krd[u] + (((4 * s + g) ^ fc) << 4));
-#pragma unroll
-                for (int x = 0; x < RT; x++) st[x][u] = mma16<T>(kf, qf[x][s], st[x][u]);
-            }
+            for (int u = 0; u < 2; u++)
+                st[u] = mma16<T>(*(const V8 *)(sk + krd[u] + (((4 * s + g) ^ fc) << 4)), qf[s], st[u]);
         if (more) {
             next = key_tile(a, k, list, t + WV);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its reads are done
             load_k(next);
         }
-        V8 pb[RT];
+        float tv[8];
 #pragma unroll
-        for (int x = 0; x < RT; x++) {
-            float tv[8];
+        for (int i = 0; i < 8; i++) tv[i] = st[i >> 2][i & 3];
+        if (now.n < 32 || (!now.pre && a.causal)) {
+            const int top = now.pre ? now.n - 1 : min(last - now.key0, now.n - 1);
 #pragma unroll
-            for (int i = 0; i < 8; i++) tv[i] = st[x][i >> 2][i & 3];
-            if (now.n < 32 || (!now.pre && a.causal)) {
-                const int top = now.pre ? now.n - 1 : min(last[x] - now.key0, now.n - 1);
+            for (int i = 0; i < 8; i++)
+                if (8 * g + i > top) tv[i] = -INFINITY;
+        }
+        float mloc = tv[0];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (8 * g + i > top) tv[i] = -INFINITY;
-            }
-            float mloc = tv[0];
+        for (int i = 1; i < 8; i++) mloc = fmaxf(mloc, tv[i]);
+        mloc = fmaxf(mloc, xor_lane<16>(mloc));
+        mloc = fmaxf(mloc, xor_lane<32>(mloc));
+        const float mc = mloc * a.c2;
+        const bool moved = mc > mrun + kTau;
+        if (__any(moved)) {
+            const float alpha = moved ? __builtin_amdgcn_exp2f(mrun - mc) : 1.f;
+            mrun = moved ? mc : mrun;
+            lrun *= alpha;
 #pragma unroll
-            for (int i = 1; i < 8; i++) mloc = fmaxf(mloc, tv[i]);
-            mloc = fmaxf(mloc, xor_lane<16>(mloc));
-            mloc = fmaxf(mloc, xor_lane<32>(mloc));
-            const float mc = mloc * a.c2;
-            const bool moved = mc > mrun[x] + kTau;
-            if (__any(moved)) {
-                const float alpha = moved ? __builtin_amdgcn_exp2f(mrun[x] - mc) : 1.f;
-                mrun[x] = moved ? mc : mrun[x];
-                lrun[x] *= alpha;
+            for (int i = 0; i < NO; i++) o[i] *= alpha;
+        }
+        const float ms = mrun == -INFINITY ? 0.f : mrun;
+        V8 pb;
 #pragma unroll
-                for (int i = 0; i < NO; i++) o[x][i] *= alpha;
-            }
-            const float ms = mrun[x] == -INFINITY ? 0.f : mrun[x];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(tv[i], a.c2, -ms));
-                lrun[x] += p;
-                pb[x][i] = (T)p;
-            }
+        for (int i = 0; i < 8; i++) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(tv[i], a.c2, -ms));
+            lrun += p;
+            pb[i] = (T)p;
         }
         // the tile's V^T has landed (the next K was requested after it)
         if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
@@ -368,11 +356,7 @@ __global__ __launch_bounds__((64 * FewTile<D, RT>::WV)) void k_keys_few(KeysArgs
             }
         }
 #pragma unroll
-        for (int i = 0; i < NO; i++) {
-            const V8 vf = *(const V8 *)(sv + vrd + i * 1024);
-#pragma unroll
-            for (int x = 0; x < RT; x++) o[x][i] = mma16<T>(vf, pb[x], o[x][i]);
-        }
+        for (int i = 0; i < NO; i++) o[i] = mma16<T>(*(const V8 *)(sv + vrd + i * 1024), pb, o[i]);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             load_v(next);
@@ -380,23 +364,19 @@ __global__ __launch_bounds__((64 * FewTile<D, RT>::WV)) void k_keys_few(KeysArgs
     }
 
     // join the waves: contexts as they are, with their maxima and sums; a quad of dims a thread
-#pragma unroll
-    for (int x = 0; x < RT; x++) {
-        float lsum = lrun[x] + xor_lane<16>(lrun[x]);
-        lsum += xor_lane<32>(lsum);
-        if (g == 0) s_m[w][16 * x + c] = mrun[x], s_l[w][16 * x + c] = lsum;
-    }
+    float lsum = lrun + xor_lane<16>(lrun);
+    lsum += xor_lane<32>(lsum);
+    if (g == 0) s_m[w][c] = mrun, s_l[w][c] = lsum;
     __syncthreads();  // the tiles are read
     float *ctx = (float *)few_smem;
+    {
+        float *y = ctx + (w * 16 + c) * PITCH + 4 * g;
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        float *y = ctx + (w * ROWS + 16 * x + c) * PITCH + 4 * g;
-#pragma unroll
-        for (int i = 0; i < NO; i++) *(f4v *)(y + 16 * i) = o[x][i];
+        for (int i = 0; i < NO; i++) *(f4v *)(y + 16 * i) = o[i];
     }
     __syncthreads();
 #pragma unroll 1
-    for (int at = tid; at < ROWS * D / 4; at += 64 * WV) {
+    for (int at = tid; at < 4 * D; at += 64 * WV) {
         const int row = at / (D / 4), d = at % (D / 4) * 4, r = k.r0 + row;
         float mall = s_m[0][row];
 #pragma unroll
@@ -406,7 +386,7 @@ __global__ __launch_bounds__((64 * FewTile<D, RT>::WV)) void k_keys_few(KeysArgs
 #pragma unroll
         for (int x = 0; x < WV; x++) {
             const float mx = s_m[x][row], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mall);
-            v += *(const f4v *)(ctx + (x * ROWS + row) * PITCH + d) * f;
+            v += *(const f4v *)(ctx + (x * 16 + row) * PITCH + d) * f;
             sum += s_l[x][row] * f;
         }
         if (sum != sum) v = (f4v)NAN;
@@ -914,7 +894,7 @@ __global__ __launch_bounds__(256) void k_keys_merge(KeysArgs a) {
 
 // ---- host: plan, checks, launches
 
-// How a set of rows runs: k_keys_few with tiles of 16 (nw 0) or 32 rows (nw 1), else k_keys_wide with nw row groups of 32.
+// How a set of rows runs: nw 0: k_keys_few, else k_keys_wide with nw row groups of 32.
 struct RowsPlan {
     int nw = 0, parts = 1;
     int64_t tiles = 0;  // per sequence and kv head
@@ -939,22 +919,30 @@ static int key_shares(int64_t groups, int64_t tiles, int per, int least, int mos
 // k_keys_wide's offsets into V^T within a wave's rows (up to 128) are 32 bits: caches past 8 M columns take k_keys_few
 static bool wide_takes(const KeySet &s) { return !s.rows || s.ldv < (1 << 23); }
 
-// groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles
+// Bytes of K and V^T that k_keys_few would ask for: each of its tiles of 16 rows reads every key tile.
+static double few_bytes(int64_t rows, int64_t count, int64_t tiles, int D) { return (double)((rows + 15) / 16 * count) * tiles * 128 * D; }
+
+// Groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles. Which kernel: few rows are
+// faster where the keys that its tiles ask for again come from L2 in about the time of the launch, and a group of 16
+// rows or fewer asks once anyway. us a call, k_keys_few | k_keys_wide, by those bytes (4 heads on 1 kv head):
+//   head_dim 128:  268 MB (2048 tokens in blocks of 8, 16 blocks of keys) 21.5 | 29.9, 1070 MB (8192 tokens) 74.6 | 44.8
+//   head_dim 256:  136 MB (128 tokens behind 4096 keys) 21.4 | 25.0, 537 MB (2048 tokens in blocks of 8) 41.6 | 39.0
+//   head_dim 512:   68 MB (32 tokens behind 4096 keys) 27.9 | 29.8, 136 MB (64 tokens) 34.7 | 30.0, one group of 16 rows
+//   of many, 4300 MB: 519 | 440
 static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int most, bool wide, bool joined) {
     RowsPlan p;
-    p.nw = rows <= 16 ? 0 : rows <= 32 ? (D < 512 ? 1 : 0) : rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
-    // Rows that cannot fill the device in tiles of 128 even in shares: tiles of 32 with 128 KB of keys in flight a CU beat
-    // them by reading the keys several times (from L2). 64 streams of 4 heads on 2 kv heads behind 16384 keys, head_dim
-    // 256, us of the prefix's launch: XX | YY.
-    if (!wide && p.nw >= 2) p.nw = D < 512 ? 1 : 0;
-    if (p.nw >= 2 && D < 512 && (rows + 127) / 128 * count * 32 < num_cus()) p.nw = 1;
+    p.nw = rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
+    // two row groups where four would not give every CU a workgroup even in shares (head_dim 512, 64 tokens behind 4096 keys:
+    // 30.0 | 38.0 with four)
+    if ((rows + 127) / 128 * count * std::min<int64_t>(most, std::max<int64_t>(1, tiles / 8)) < num_cus()) p.nw = 2;
+    if (!wide || few_bytes(rows, count, tiles, D) <= (D < 512 ? 400e6 : 100e6) || (rows <= 16 && D < 512)) p.nw = 0;
     const int R = p.nw ? 32 * p.nw : 16;
     p.tiles = (rows + R - 1) / R;
     // k_keys_few fills a CU's LDS from head_dim 256 on
-    p.parts = key_shares(p.tiles * count, tiles, p.nw >= 2 || D < 256 ? 2 : 1, p.nw >= 2 ? 8 : 4, most);
+    p.parts = key_shares(p.tiles * count, tiles, p.nw || D < 256 ? 2 : 1, p.nw ? 8 : 4, most);
     // up to six tiles a wave, one workgroup's walk is shorter than a second launch to join shares (one token of 3 heads over
     // 531 keys of 256, us a call: 12.9 | 16.1 in four shares), unless there is one anyway (`joined`)
-    if (p.nw < 2 && tiles <= 24 && !joined) p.parts = 1;
+    if (!p.nw && tiles <= 24 && !joined) p.parts = 1;
     return p;
 }
 
@@ -967,8 +955,10 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
     const int G = H / KV, P = pre.rows;
     const int64_t own_tiles = own.rows ? ((int64_t)max_k + 31) / 32 : 0, pre_tiles = ((int64_t)P + 31) / 32;
     const int64_t rows = (int64_t)max_q * G;
-    // sequences of less than a tile share the prefix's tiles
-    p.apart = B > 1 && P > 0 && rows < 32;
+    // Sequences of few rows share the prefix's tiles where reading it for each costs more than the join of the shares, which
+    // follows the rows' contexts. us a call, each | shared: head_dim 256, 64 sequences of 1 token of 4 heads behind 2048 keys
+    // 19.2 | 21.3, 4096 25.4 | 23.7, 16384 62.6 | 33.3; of 8 tokens 2048 27.1 | 36.8, 8192 62.7 | 55.2.
+    p.apart = B > 1 && P > 0 && rows <= 64 && few_bytes(rows, (int64_t)B * KV, pre_tiles, D) > 200e6 + 1400.0 * Mq * H * D;
     if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, D, kMaxKeyParts / 2, wide_takes(pre), true);
     p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), D, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts,
                        wide_takes(own) && (p.apart || wide_takes(pre)), p.apart);
@@ -1001,12 +991,12 @@ static int launch_wide(hipStream_t st, const KeysArgs &a, int64_t tiles, int64_t
     return check_hip(hipGetLastError(), "attention launch");
 }
 
-template <class T, int D, int RT>
+template <class T, int D>
 static int launch_few(hipStream_t st, const KeysArgs &a, int64_t grid, int B) {
-    const size_t lds = FewTile<D, RT>::kBytes + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
+    const size_t lds = FewTile<D>::kBytes + (a.mode == kSelected ? 4 * (size_t)a.n_sel : 0);
     static LdsAllowed allowed;
-    if (allow_lds((const void *)k_keys_few<T, D, RT>, (int)lds, allowed)) return -1;
-    hipLaunchKernelGGL((k_keys_few<T, D, RT>), dim3((unsigned)grid, a.KV, B), dim3(64 * FewTile<D, RT>::WV), lds, st, a);
+    if (allow_lds((const void *)k_keys_few<T, D>, (int)lds, allowed)) return -1;
+    hipLaunchKernelGGL((k_keys_few<T, D>), dim3((unsigned)grid, a.KV, B), dim3(64 * FewTile<D>::WV), lds, st, a);
     return check_hip(hipGetLastError(), "attention launch");
 }
 
@@ -1021,9 +1011,7 @@ static int launch_rows(hipStream_t st, KeysArgs a, const RowsPlan &p, int B) {
     if (p.nw == 2) return launch_wide<T, D, 2>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 3) return launch_wide<T, D, 3>(st, a, p.tiles, grid * a.KV * B);
     if (p.nw == 4) return launch_wide<T, D, 4>(st, a, p.tiles, grid * a.KV * B);
-    // head_dim 512 has no registers for two tiles of rows
-    if (D < 512 && p.nw == 1) return launch_few<T, D, D < 512 ? 2 : 1>(st, a, grid, B);
-    return launch_few<T, D, 1>(st, a, grid, B);
+    return launch_few<T, D>(st, a, grid, B);
 }
 // a copy of a set's V^T in rows of 16-byte multiples at `to` (columns past its rows: zeros)
 static int pad_values(hipStream_t st, KeySet &s, int KV, int D, uint16_t *to) {
