@@ -976,6 +976,20 @@ static KeysPlan plan_blocks(const KeySet &own, int B, int max_q, int H, int KV, 
     return p;
 }
 
+// The plans as tests read them: {apart, the prefix's launch: nw, shares, the other launch: nw, shares, copies of V^T}; nw 0 is
+// k_keys_few.
+static void plan_out(const KeysPlan &p, int *out) {
+    const int v[6] = {p.apart, p.pre.nw, p.apart ? p.pre.parts : 0, p.rows.nw, p.rows.parts, (p.pad_pre != 0) + (p.pad_own != 0)};
+    for (int i = 0; i < 6; i++) out[i] = v[i];
+}
+void keys_route_prefix(int Mq, int Mk, int P, int B, int max_q, int max_k, int H, int KV, int D, int *out) {
+    plan_out(plan_prefix(Mq, {nullptr, nullptr, 0, (Mk + 7) / 8 * 8, Mk}, {nullptr, nullptr, 0, (P + 7) / 8 * 8, P}, B, max_q, max_k, H, KV, D),
+             out);
+}
+void keys_route_blocks(int Mk, int B, int max_q, int H, int KV, int D, int q_block, int n_sel, int *out) {
+    plan_out(plan_blocks({nullptr, nullptr, 0, (Mk + 7) / 8 * 8, Mk}, B, max_q, H, KV, D, q_block, n_sel), out);
+}
+
 static size_t part_bytes(const KeysPlan &p, int Mq, int H, int D) {
     return p.all() > 1 ? ((size_t)p.all() * Mq * H * (D + 2) * 4 + 15) / 16 * 16 : 0;
 }
@@ -1173,7 +1187,7 @@ extern "C" int e2mi_attention_blocks(e2mi_stream stream, int dtype, const uint16
         return -1;
     }
     if (!Mq || !B || !max_q) return 0;
-    a.NQ = (max_q + q_block - 1) / q_block;
+    a.NQ = (int)(((int64_t)max_q + q_block - 1) / q_block);
     const KeysPlan p = plan_blocks(a.own, B, max_q, H, KV, D, q_block, n_sel);
     if (check_workspace("attention_blocks", workspace_of(p, Mq, H, D), workspace, workspace_bytes)) return -1;
     return run_keys((hipStream_t)stream, dtype, D, a, p, workspace);

@@ -531,16 +531,16 @@ extern "C" int e2mi_block_select(e2mi_stream stream, int dtype, const uint16_t *
     SelectArgs a = {};
     a.q = q, a.ldq = ldq, a.Mq = Mq, a.bounds = bounds, a.kscale = scale, a.q_start = q_start, a.q_len = q_len, a.k_len = k_len;
     a.max_q = max_q, a.max_k = max_k, a.KV = KV, a.G = G, a.NB = (max_k + kKeyBlock - 1) / kKeyBlock;
-    a.NQ = (max_q + q_block - 1) / q_block, a.q_block = q_block, a.n_sel = n_sel, a.n_first = n_first, a.n_local = n_local;
+    a.NQ = (int)(((int64_t)max_q + q_block - 1) / q_block), a.q_block = q_block, a.n_sel = n_sel, a.n_first = n_first, a.n_local = n_local;
     a.causal = causal != 0, a.scores = (float *)workspace, a.sel = sel;
     a.group = R <= 4 ? 4 : R <= 8 ? 8 : R <= 16 ? 16 : 32;
     const hipStream_t st = (hipStream_t)stream;
-    if (a.NB && Mq && E2MI_BY_TYPE(launch_scores, dtype, D, st, a, B)) return -1;
     const int64_t lists = (int64_t)B * a.NQ * KV;
     if (lists > 0x7fffffff) {
         set_error("block_select: too many lists for a launch");
         return -1;
     }
+    if (a.NB && Mq && E2MI_BY_TYPE(launch_scores, dtype, D, st, a, B)) return -1;
     const unsigned n = (unsigned)lists;
     // a wave a list, keys in registers; past 1024 blocks four where the lists are too few to fill the device
     const bool few = lists < 4L * num_cus();

@@ -59,44 +59,54 @@ def make(dev, seed, dtype, H, KV, D, q_lens, k_lens, P=0, lead=8, spread=1.0):
     return c
 
 
+def reference(c, scale, causal, keys_of=None, q_block=None):
+    """64-bit context and tolerance [Mq, H * D] (zeros outside the sequences), on the tensors' device. keys_of(b, block, kv head):
+    the own keys (in any order, a key twice counts twice) that the block of q_block queries reads; None: all."""
+    import torch
+    H, KV, D, G = c["H"], c["KV"], c["D"], c["H"] // c["KV"]
+    dev = c["q"].device
+    f64 = dict(dtype=torch.float64, device=dev)
+    u = U[c["dtype"]]
+    y, tol = torch.zeros((c["Mq"], H * D), **f64), torch.zeros((c["Mq"], H * D), **f64)
+    P = 0 if c["pk"] is None else c["pk"].shape[0]
+    for b, (q0, k0, nq, nk) in enumerate(zip(c["qs"], c["ks"], c["q_lens"], c["k_lens"])):
+        step = q_block or max(nq, 1)
+        for a in range(KV):
+            kk = [] if c["k"] is None else [c["k"][k0:k0 + nk, a * D:(a + 1) * D].double()]
+            vv = [] if c["k"] is None else [c["vt"][a, :, k0:k0 + nk].double().T]
+            if P:
+                kk, vv = [c["pk"][:, a * D:(a + 1) * D].double()] + kk, [c["pvt"][a].double().T] + vv
+            if not kk:
+                continue
+            kk, vv = torch.cat(kk).contiguous(), torch.cat(vv).contiguous()
+            for i in range(0, nq, step):
+                n = min(step, nq - i)
+                own = torch.arange(nk, device=dev) if keys_of is None else torch.as_tensor(keys_of(b, i // step, a), dtype=torch.int64, device=dev)
+                own = own[own < nk]
+                at = torch.cat([torch.arange(P, device=dev), P + own])
+                if not at.numel():
+                    continue
+                rows = c["q"][q0 + i:q0 + i + n].double().view(n, H, D)[:, a * G:(a + 1) * G].reshape(n * G, D)
+                k, v = kk[at], vv[at]
+                x = scale * (rows @ k.T.contiguous())
+                last = (torch.arange(i, i + n, device=dev) + nk - nq if causal else torch.full((n,), nk, device=dev)).repeat_interleave(G)
+                see = (at[None] < P) | (at[None] - P <= last[:, None])
+                x = x.masked_fill(~see, -float("inf"))
+                some = see.any(1, keepdim=True)
+                L = (D + 4) * 2.0 ** -24 * scale * (rows.abs() @ k.abs().T.contiguous()).amax(1, keepdim=True)
+                p = torch.exp(x - x.amax(1, keepdim=True).masked_fill(~some, 0.0))
+                p = p / p.sum(1, keepdim=True).masked_fill(~some, 1.0)
+                A, o = p @ v.abs(), p @ v
+                t = A * (u + 2 * L + (at.numel() + 64) * 2.0 ** -24) + u * o.abs()
+                if c["dtype"] == "float16":
+                    t = t + (at.numel() * 2.0 ** -25 * v.abs().max() + 2.0 ** -25) * some
+                y[q0 + i:q0 + i + n, a * G * D:(a + 1) * G * D] = o.reshape(n, G * D)
+                tol[q0 + i:q0 + i + n, a * G * D:(a + 1) * G * D] = t.reshape(n, G * D)
+    return y.cpu().numpy(), tol.cpu().numpy()
+
+
 def _f64(t):
     return t.double().cpu().numpy()
-
-
-def reference(c, scale, causal, keys_of=None):
-    """64-bit context and tolerance [Mq, H * D] (zeros outside the sequences). keys_of(b, token, kv head): the own
-    keys a token reads, in any order (None: all)."""
-    H, KV, D, G = c["H"], c["KV"], c["D"], c["H"] // c["KV"]
-    q, k, vt = _f64(c["q"]), _f64(c["k"]), _f64(c["vt"])
-    P = 0 if c["pk"] is None else c["pk"].shape[0]
-    pk, pvt = (_f64(c["pk"]), _f64(c["pvt"])) if P else (np.zeros((0, KV * D)), np.zeros((KV, D, 0)))
-    u = U[c["dtype"]]
-    y, tol = np.zeros((c["Mq"], H * D)), np.zeros((c["Mq"], H * D))
-    for b, (q0, k0, nq, nk) in enumerate(zip(c["qs"], c["ks"], c["q_lens"], c["k_lens"])):
-        for a in range(KV):
-            kk = np.concatenate([pk[:, a * D:(a + 1) * D], k[k0:k0 + nk, a * D:(a + 1) * D]])
-            vv = np.concatenate([pvt[a].T, vt[a, :, k0:k0 + nk].T])
-            for i in range(nq):
-                own = np.arange(nk) if keys_of is None else np.asarray(keys_of(b, i, a), dtype=np.int64)
-                own = own[own < nk]
-                if causal:
-                    own = own[own <= i + nk - nq]
-                at = np.concatenate([np.arange(P), P + own])
-                if not at.size:
-                    continue
-                rows = q[q0 + i].reshape(H, D)[a * G:(a + 1) * G]
-                x = scale * rows @ kk[at].T
-                L = (D + 4) * 2.0 ** -24 * scale * (np.abs(rows) @ np.abs(kk[at]).T).max(1, keepdims=True)
-                p = np.exp(x - x.max(1, keepdims=True))
-                p /= p.sum(1, keepdims=True)
-                A = p @ np.abs(vv[at])
-                o = p @ vv[at]
-                t = A * (u + 2 * L + (at.size + 64) * 2.0 ** -24) + u * np.abs(o)
-                if c["dtype"] == "float16":
-                    t = t + at.size * 2.0 ** -25 * np.abs(vv[at]).max() + 2.0 ** -25
-                y[q0 + i, a * G * D:(a + 1) * G * D] = o.ravel()
-                tol[q0 + i, a * G * D:(a + 1) * G * D] = t.ravel()
-    return y, tol
 
 
 def check(c, got, want, tol):
@@ -107,3 +117,23 @@ def check(c, got, want, tol):
     off = np.abs(g - want)[live]
     t = (tol * (1 + U[c["dtype"]]))[live]
     assert off.size == 0 or np.all(off <= t), f"worst {np.max(off - t)} over the tolerance; largest off {np.nanmax(off)}"
+
+
+def route_prefix(c):
+    """{apart, prefix: nw, shares, own keys: nw, shares, copies} that a call on c's sizes takes (attn_keys.hip)."""
+    import ctypes as C
+    import e2mi
+    out = (C.c_int * 6)()
+    e2mi.load()._ZN4e2mi17keys_route_prefixEiiiiiiiiiPi(c["Mq"], 0 if c["k"] is None else c["k"].shape[0],
+                                                        0 if c["pk"] is None else c["pk"].shape[0], len(c["q_lens"]), c["max_q"],
+                                                        c["max_k"], c["H"], c["KV"], c["D"], out)
+    return list(out)
+
+
+def route_blocks(c, q_block, n_sel):
+    import ctypes as C
+    import e2mi
+    out = (C.c_int * 6)()
+    e2mi.load()._ZN4e2mi17keys_route_blocksEiiiiiiiiPi(c["k"].shape[0], len(c["q_lens"]), c["max_q"], c["H"], c["KV"], c["D"], q_block,
+                                                       n_sel, out)
+    return list(out)

@@ -130,10 +130,10 @@ def test_attention_over_lists(gpu, case, causal):
     s = sel.cpu().numpy()
 
     def keys(b, i, a):
-        blocks = s[b, i // qb, a]
+        blocks = s[b, i, a]
         return [64 * n + j for n in blocks[blocks >= 0] for j in range(64)]
 
-    check(c, _attend(c, sel, qb, D ** -0.5, causal), *reference(c, D ** -0.5, causal, keys))
+    check(c, _attend(c, sel, qb, D ** -0.5, causal), *reference(c, D ** -0.5, causal, keys, qb))
 
 
 def test_every_block_listed_is_the_whole_attention(gpu):
@@ -157,9 +157,9 @@ def test_lists_of_a_callers_own(gpu):
     read = {(0, 0): [4, 0], (0, 1): [2, 2], (1, 0): [], (1, 1): [1, 0, 3, 3]}
 
     def keys(b, i, a):
-        return [64 * n + j for n in read[i // 32, a] for j in range(64)]
+        return [64 * n + j for n in read[i, a] for j in range(64)]
 
-    check(c, _attend(c, sel, 32, 0.1), *reference(c, 0.1, False, keys))
+    check(c, _attend(c, sel, 32, 0.1), *reference(c, 0.1, False, keys, 32))
 
 
 def test_ties_and_order(gpu):
@@ -254,10 +254,10 @@ def test_together_after_rope(gpu):
         assert np.array_equal(lists, select_of(c, bounds_of(c), qb, n_sel, 1, 1, True))
 
         def keys(b, i, a):
-            blocks = lists[b, i // qb, a]
+            blocks = lists[b, i, a]
             return [64 * n + j for n in blocks[blocks >= 0] for j in range(64)]
 
-        check(c, got, *reference(c, D ** -0.5, True, keys))
+        check(c, got, *reference(c, D ** -0.5, True, keys, qb))
 
 
 def test_a_prefix_turned_once(gpu):
