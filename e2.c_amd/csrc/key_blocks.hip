@@ -516,7 +516,7 @@ extern "C" int e2mi_block_select(e2mi_stream stream, int dtype, const uint16_t *
                   n_first, n_local, n_sel);
         return -1;
     }
-    if (!q || !aligned16(q) || ldq < (int64_t)H * D || ldq % 8 || ldq > (1LL << 28) || !q_start || !q_len || !k_len || !sel ||
+    if ((Mq && (!q || !aligned16(q))) || ldq < (int64_t)H * D || ldq % 8 || ldq > (1LL << 28) || !q_start || !q_len || !k_len || !sel ||
         (max_k && (!bounds || !scale || !aligned16(bounds)))) {
         set_error("block_select: needs row ranges, 16-byte aligned q rows (pitch >= H * D in multiples of 8), bounds, scales and sel");
         return -1;

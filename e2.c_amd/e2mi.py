@@ -788,6 +788,13 @@ def _rows(name, t, rows, width, dtype, dev):
     return t.data_ptr(), stride[0] if rows > 1 else max(stride[0], width)
 
 
+def _head_dim(name, t, H, KV):
+    """The head dim of rows [.., H * D] on KV kv heads."""
+    if len(t.shape) != 2 or H <= 0 or KV <= 0 or t.shape[1] % H:
+        raise E2MIError(f"{name}: needs rows of H heads on KV kv heads, got {tuple(t.shape)}, H={H}, KV={KV}")
+    return t.shape[1] // H
+
+
 def _indices(name, t, n, dev):
     """Address of a contiguous int32 device array of at least n entries."""
     import torch
@@ -811,9 +818,10 @@ def rope_freqs(rot_dim, theta=10000.0, scaling="plain", factor=1.0, trained_len=
     "linear", "base" or "parts"."""
     import numpy as np
     import torch
+    if scaling not in _SCALINGS:
+        raise E2MIError(f"rope_freqs: scaling {scaling!r}, not one of {', '.join(_SCALINGS)}")
     f = np.empty(max(1, rot_dim // 2), np.float64)
-    kind = {"plain": 0, "linear": 1, "base": 2, "parts": 3}[scaling]
-    check(load().e2mi_rope_freqs(ptr(f), rot_dim, theta, kind, factor, trained_len, turns[0], turns[1]), "rope_freqs")
+    check(load().e2mi_rope_freqs(ptr(f), rot_dim, theta, _SCALINGS[scaling], factor, trained_len, turns[0], turns[1]), "rope_freqs")
     return torch.from_numpy(f)
 
 
@@ -825,11 +833,11 @@ def rope(q, k, pos, freqs, H, KV, layout="half", magnitude=1.0, inverse=False, q
     x, heads = (q, H) if q is not None else (k, KV)
     if x is None:
         raise E2MIError("rope: needs q or k")
+    if layout not in _LAYOUTS:
+        raise E2MIError(f"rope: layout {layout!r}, not one of {', '.join(_LAYOUTS)}")
+    D = _head_dim("rope", x, heads, heads)
     kind, dev = _kind("rope", x)
     dtype, (M, width) = x.dtype, x.shape
-    if heads <= 0 or width % heads:
-        raise E2MIError(f"rope: {width} values are not {heads} heads")
-    D = width // heads
     pq = pk = po = pt = None
     lq = lk = lo = lt = nq = nk = 0
     if q is not None:
@@ -850,12 +858,15 @@ def rope(q, k, pos, freqs, H, KV, layout="half", magnitude=1.0, inverse=False, q
             pt, lt = _rows("rope", k_out, M, KV * D, dtype, dev)
     if freqs.dtype is not torch.float64 or freqs.get_device() != dev or not freqs.is_contiguous():
         raise E2MIError(f"rope: needs contiguous float64 frequencies on device {dev}")
+    if not M:  # an empty tensor has no address
+        return q_out, k_out
     check(load().e2mi_rope(_stream(stream), kind, _LAYOUTS[layout], 1 if inverse else 0, pq, lq, po, lo, nq, pk, lk, pt, lt, nk, M,
                            D, _indices("rope", pos, M, dev), freqs.data_ptr(), 2 * freqs.numel(), magnitude), "rope")
     return q_out, k_out
 
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
+_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "parts": 3}
 _NO_KEYS = (None, 0, None, 0, 0)
 
 
@@ -914,9 +925,10 @@ def attention_prefix(q, k, vt, pk, pvt, q_start, q_len, max_q, H, KV, k_start=No
     [KV, D, >= P] (None: none); ranges int32 [B] on the device, key ranges those of q unless given. Returns
     ctx [Mq, H * D] (new unless given), or with quant the pair (int8 [Mq, H * D], f32 scales per 128)."""
     name = "attention_prefix"
+    D = _head_dim(name, q, H, KV)
     kind, dev = _kind(name, q)
     Mq, width = q.shape
-    dtype, B, D = q.dtype, q_start.shape[0], width // H
+    dtype, B = q.dtype, q_start.shape[0]
     pq, lq = _rows(name, q, Mq, H * D, dtype, dev)
     own, pre = _keys(name, k, vt, KV, D, dtype, dev), _keys(name, pk, pvt, KV, D, dtype, dev)
     qs, ql = _indices(name, q_start, B, dev), _indices(name, q_len, B, dev)
@@ -924,6 +936,8 @@ def attention_prefix(q, k, vt, pk, pvt, q_start, q_len, max_q, H, KV, k_start=No
     kl = ql if k_len is None else _indices(name, k_len, B, dev)
     max_k = max_q if max_k is None else max_k
     ctx, pc, lc, pair, cq, cs = _context(name, q, Mq, width, ctx, quant, stream, dev)
+    if not (Mq and B):
+        return pair if quant else ctx
     ws, pw, nw = _workspace(name, _workspace_bytes(name, dev, Mq, own[4], own[3], pre[4], pre[3], B, max_q, max_k, H, KV, D),
                             workspace, q, stream, dev)
     check(load().e2mi_attention_prefix(_stream(stream), kind, pq, lq, Mq, *own, *pre, qs, ql, ks, kl, B, max_q, max_k, H, KV, D,
@@ -947,14 +961,16 @@ def block_bounds(k, k_start, k_len, max_k, KV, bounds=None, stream=None):
     new unless given. Blocks past a sequence's keys are left as they are."""
     import torch
     name = "block_bounds"
+    D = _head_dim(name, k, KV, KV)
     kind, dev = _kind(name, k)
-    Mk, width = k.shape
-    D, B, NB = width // KV, k_start.shape[0], (max_k + 63) // 64
+    Mk, B, NB = k.shape[0], k_start.shape[0], (max_k + 63) // 64
     pk, lk = _rows(name, k, Mk, KV * D, k.dtype, dev)
     if bounds is None:
         bounds = (_new(stream, torch.empty, (B, NB, KV, 2 * D), dtype=torch.int8, device=k.device),
                   _new(stream, torch.empty, (B, NB, KV), dtype=torch.float32, device=k.device))
     pb, ps = _bounds(name, bounds, B, NB, KV, D, dev)
+    if not (Mk and B and NB):
+        return bounds
     check(load().e2mi_block_bounds(_stream(stream), kind, pk, lk, Mk, _indices(name, k_start, B, dev), _indices(name, k_len, B, dev),
                                    B, max_k, KV, D, pb, ps), name)
     return bounds
@@ -966,9 +982,9 @@ def block_select(q, bounds, q_start, q_len, k_len, max_q, max_k, H, KV, q_block,
     [B, ceil(max_q / q_block), KV, n_sel], ascending, -1 past the last."""
     import torch
     name = "block_select"
+    D = _head_dim(name, q, H, KV)
     kind, dev = _kind(name, q)
-    Mq, width = q.shape
-    D, B = width // H, q_start.shape[0]
+    Mq, B = q.shape[0], q_start.shape[0]
     pq, lq = _rows(name, q, Mq, H * D, q.dtype, dev)
     pb, ps = _bounds(name, bounds, B, (max_k + 63) // 64, KV, D, dev)
     if q_block <= 0 or n_sel <= 0:
@@ -978,6 +994,8 @@ def block_select(q, bounds, q_start, q_len, k_len, max_q, max_k, H, KV, q_block,
         sel = _new(stream, torch.empty, shape, dtype=torch.int32, device=q.device)
     elif sel.shape != shape:
         raise E2MIError(f"{name}: needs sel {shape}, got {tuple(sel.shape)}")
+    if not (B and max_q):
+        return sel
     ws, pw, nw = _workspace(name, _workspace_bytes(name, dev, B, max_q, max_k, KV, q_block), workspace, q, stream, dev)
     check(load().e2mi_block_select(_stream(stream), kind, pq, lq, Mq, pb, ps, _indices(name, q_start, B, dev),
                                    _indices(name, q_len, B, dev), _indices(name, k_len, B, dev), B, max_q, max_k, H, KV, D, q_block,
@@ -990,15 +1008,18 @@ def attention_blocks(q, k, vt, sel, q_start, q_len, k_start, k_len, max_q, max_k
     """Attention over the listed blocks of 64 keys (e2mi_attention_blocks): sel as block_select gives it. Returns as
     attention_prefix."""
     name = "attention_blocks"
+    D = _head_dim(name, q, H, KV)
     kind, dev = _kind(name, q)
     Mq, width = q.shape
-    dtype, B, D = q.dtype, q_start.shape[0], width // H
+    dtype, B = q.dtype, q_start.shape[0]
     pq, lq = _rows(name, q, Mq, H * D, dtype, dev)
     own = _keys(name, k, vt, KV, D, dtype, dev)
     if q_block <= 0 or sel.dim() != 4 or sel.shape[:3] != (B, (max_q + q_block - 1) // q_block, KV):
         raise E2MIError(f"{name}: needs q_block of at least 1 and sel [{B}, query blocks, {KV}, n], got {q_block}, {tuple(sel.shape)}")
     n_sel = sel.shape[3]
     ctx, pc, lc, pair, cq, cs = _context(name, q, Mq, width, ctx, quant, stream, dev)
+    if not (Mq and B):
+        return pair if quant else ctx
     ws, pw, nw = _workspace(name, _workspace_bytes(name, dev, Mq, own[4], own[3], B, max_q, H, KV, D, q_block, n_sel), workspace, q,
                             stream, dev)
     check(load().e2mi_attention_blocks(_stream(stream), kind, pq, lq, Mq, *own, _indices(name, q_start, B, dev),

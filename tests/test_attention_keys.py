@@ -84,3 +84,18 @@ def test_workspace_sizes():
     for over in (dict(ws=None, wn=0), dict(wn=need - 1), dict(ws=X + 4)):
         assert lib.e2mi_attention_prefix(*{**few, **over}.values()) == -1
         assert "workspace" in e2mi.last_error()
+
+
+def test_wrapper_refusals_need_no_gpu():
+    import e2mi
+    import torch
+    x, i = torch.zeros(8, 512, dtype=torch.float16), torch.zeros(1, dtype=torch.int32)
+    for H, KV in ((0, 1), (2, 0), (-2, 1), (3, 1)):
+        with pytest.raises(e2mi.E2MIError, match="attention_prefix"):
+            e2mi.attention_prefix(x, None, None, None, None, i, i, 8, H, KV)
+        with pytest.raises(e2mi.E2MIError, match="attention_blocks"):
+            e2mi.attention_blocks(x, x, x, i, i, i, i, i, 8, 8, H, KV, 4)
+        with pytest.raises(e2mi.E2MIError, match="block_select"):
+            e2mi.block_select(x, (x, x), i, i, i, 8, 8, H, KV, 4, 2)
+    with pytest.raises(e2mi.E2MIError, match="block_bounds"):
+        e2mi.block_bounds(x, i, i, 8, 0)

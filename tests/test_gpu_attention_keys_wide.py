@@ -164,3 +164,41 @@ def test_caches_past_the_wide_kernels_offsets(gpu):
     k[k0:k0 + 2000] = c["k"][c["ks"][0]:c["ks"][0] + 2000]
     c["k"], c["vt"], c["k_start"] = k, vt, torch.tensor([k0], dtype=torch.int32, device=gpu)
     check(c, _run(c, 0.125, True), y, tol)
+
+
+def test_context_and_pair_at_once(gpu):
+    """Both outputs of one call are those of two calls, in this kernel, in shares, and in the kernel for few rows."""
+    import ctypes as C
+    import e2mi
+    import torch
+    for D, ql, P, nw in ((256, _lens(1, 3, 300, 701), 333, 4), (512, [301, 100], 777, 2), (128, [40, 3], 30, 0)):
+        c = make(gpu, 38, "float16", 4, 1, D, ql, None, P)
+        plan = route_prefix(c)
+        assert plan[3] == nw
+        ctx = _run(c, D ** -0.5).clone()
+        cq, cs = _run(c, D ** -0.5, ctx=None, quant=True)
+        got, gq, gs = torch.full_like(ctx, MARK), torch.zeros_like(cq), torch.zeros_like(cs)
+        lib, Mk, ldv = e2mi.load(), c["k"].shape[0], c["vt"].stride(1)
+        need = lib.e2mi_attention_prefix_workspace_bytes(c["Mq"], Mk, ldv, P, P, len(ql), c["max_q"], c["max_k"], 4, 1, D)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=gpu)
+        p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+        e2mi.check(lib.e2mi_attention_prefix(
+            torch.cuda.current_stream().cuda_stream, 0, p(c["q"]), 4 * D, c["Mq"], p(c["k"]), D, p(c["vt"]), ldv, Mk, p(c["pk"]), D,
+            p(c["pvt"]), P, P, p(c["q_start"]), p(c["q_len"]), p(c["k_start"]), p(c["k_len"]), len(ql), c["max_q"], c["max_k"], 4, 1, D,
+            D ** -0.5, 0, p(got), 4 * D, p(gq), p(gs), p(ws), need), "attention_prefix")
+        assert torch.equal(got, ctx) and torch.equal(gq, cq) and torch.equal(gs, cs)
+
+
+def test_empty_batches(gpu):
+    """No rows or no sequences: empty results; lists of sequences without rows: none."""
+    import e2mi
+    import torch
+    none, i32 = torch.empty(0, 512, dtype=torch.float16, device=gpu), lambda n: torch.zeros(n, dtype=torch.int32, device=gpu)  # noqa: E731
+    k, vt, some = torch.zeros(64, 256, dtype=torch.float16, device=gpu), torch.zeros(1, 256, 64, dtype=torch.float16, device=gpu), i32(2)
+    assert e2mi.attention_prefix(none, None, None, k, vt, some, some, 4, 2, 1).shape == (0, 512)
+    assert int(e2mi.attention_prefix(k, None, None, k, vt, i32(0), i32(0), 4, 1, 1).abs().max()) == 0
+    assert e2mi.rope(none, None, i32(0), torch.ones(128, dtype=torch.float64, device=gpu), 2, 0)[0].shape == (0, 512)
+    bounds = e2mi.block_bounds(k, some, some + 64, 64, 1)
+    sel = e2mi.block_select(none, bounds, some, some, some + 64, 4, 64, 2, 1, 4, 3)
+    assert sel.shape == (2, 1, 1, 3) and int(sel.max()) == -1 == int(sel.min())
+    assert e2mi.attention_blocks(none, k, vt, sel, some, some, some, some + 64, 4, 64, 2, 1, 4).shape == (0, 512)

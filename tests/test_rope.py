@@ -76,6 +76,12 @@ def test_wrapper_refusals_need_no_gpu():
     import torch
     with pytest.raises(e2mi.E2MIError, match="needs q or k"):
         e2mi.rope(None, None, None, None, 1, 1)
+    x = torch.zeros(2, 256, dtype=torch.float16)
+    for H, layout in ((0, "half"), (-1, "half"), (3, "half"), (1, "both")):
+        with pytest.raises(e2mi.E2MIError, match="rope"):
+            e2mi.rope(x, None, None, None, H, 0, layout)
+    with pytest.raises(e2mi.E2MIError, match="scaling"):
+        e2mi.rope_freqs(64, scaling="other")
     if not torch.cuda.is_available():
         return
     x = torch.zeros(2, 256, dtype=torch.float16)
