@@ -451,6 +451,7 @@ __device__ inline int spread(int i) {
 // XCDs idle.
 constexpr int kFindMost = 512;  // sequences; beyond, the sums take longer than idle workgroups
 struct LiveTiles {
+    int per;              // row tiles of a sequence and kv head (find)
     int n, sum, all, at;  // of 64 sequences from `at` on: a lane's items, with those of the lanes before, all lanes'
     __device__ inline void add(const KeysArgs &a, int R, int from) {
         const int lane = threadIdx.x & 63;
@@ -477,7 +478,8 @@ struct LiveTiles {
             if (at != b0) add(a, R, b0);
             if (item < all) {
                 const int l = __builtin_ctzll(__ballot(sum > item));
-                const int mine = __builtin_amdgcn_readlane(n, l), in = item - (__builtin_amdgcn_readlane(sum, l) - mine), per = mine / a.KV;
+                const int mine = __builtin_amdgcn_readlane(n, l), in = item - (__builtin_amdgcn_readlane(sum, l) - mine);
+                per = mine / a.KV;
                 b = b0 + l, kvh = in / per, tile = in % per;
                 return true;
             }
@@ -522,10 +524,12 @@ __global__ __launch_bounds__((64 * NW * WideTile<D, NW>::DS), 2) void k_keys_wid
     if (search) {
         if (!lt.find(a, 32 * NW, id, b, kvh, tile)) return;
     } else {
+        lt.per = tiles;
         tile = id % tiles;
         id /= tiles;
         kvh = id % a.KV, b = id / a.KV;
     }
+    if (a.causal && a.mode == kOwnRows) tile = lt.per - 1 - tile;  // the longest walks first
     Walk k;
     if (!start_walk<32 * NW>(a, kvh, b, tile, part, list, &s_count, k)) return;
     const int r1 = k.r0 + 32 * group;     // the group's first row
@@ -906,14 +910,22 @@ struct KeysPlan {
     int all() const { return (apart ? pre.parts : 0) + rows.parts; }
 };
 
-// Shares for `groups` workgroups whose longest walk is `tiles` key tiles of 32: enough to give every CU `per` workgroups, at
-// least `least` tiles each.
-static int key_shares(int64_t groups, int64_t tiles, int per, int least, int most) {
-    if (groups < 1) return 1;
-    const int64_t want = ((int64_t)per * num_cus() + groups - 1) / groups;
-    int64_t n = want < tiles / least ? want : tiles / least;
-    if (n > most) n = most;
-    return n < 1 ? 1 : (int)n;
+// Shares of the key range, of `tiles` tiles of 32, for `groups` workgroups (an estimate) where `slots` run at once, by what a
+// call takes: rounds of workgroups, each the tiles of a share and two tiles' worth of start and end, and with more than one
+// share the f32 contexts written and read again (`ctx_us` a share) and, unless it follows anyway, another launch. A round that
+// is begun is paid for: 150 groups are faster in 3 shares (450 workgroups, two rounds of a third each) than in 2 (300, two
+// rounds of a half). us a call, by the smallest number that fills the device | by this rule: one text of 1500 tokens of 4 heads
+// behind 4096 keys, head_dim 512 145 | 103, 256 73 | 59; 40 tokens of 8 heads on 4 over 8192 keys, 256 320 | 243, 128 142 | 125. Over 72 shapes it takes 1 % more than the best number of shares, the other 13 %.
+static int key_shares(double groups, int64_t tiles, int slots, double tile_us, double ctx_us, bool joined, int least, int most) {
+    const int64_t end = std::min<int64_t>(most, tiles / least);
+    int64_t best = 1;
+    double best_us = 0.;
+    for (int64_t n = 1; n <= end; n++) {
+        const double us = ceil(groups * (double)n / slots - 1e-9) * (double)((tiles + n - 1) / n + 2) * tile_us +
+                          (n > 1 || joined ? (double)n * ctx_us : 0.) + (n > 1 && !joined ? 7. : 0.);
+        if (n == 1 || us < best_us) best = n, best_us = us;
+    }
+    return (int)best;
 }
 
 // k_keys_wide's offsets into V^T within a wave's rows (up to 128) are 32 bits: caches past 8 M columns take k_keys_few
@@ -922,14 +934,15 @@ static bool wide_takes(const KeySet &s) { return !s.rows || s.ldv < (1 << 23); }
 // Bytes of K and V^T that k_keys_few would ask for: each of its tiles of 16 rows reads every key tile.
 static double few_bytes(int64_t rows, int64_t count, int64_t tiles, int D) { return (double)((rows + 15) / 16 * count) * tiles * 128 * D; }
 
-// Groups of `rows` rows (a sequence's, a query block's), `count` of them, over `tiles` key tiles. Which kernel: few rows are
+// `count` groups (sequences, query blocks; times kv heads) of at most `rows` rows over `tiles` key tiles. The lengths are on
+// the device; the host's guess is that `live` of the groups have rows, `all` together. values: of the context. Which kernel: few rows are
 // faster where the keys that its tiles ask for again come from L2 in about the time of the launch, and a group of 16
 // rows or fewer asks once anyway. us a call, k_keys_few | k_keys_wide, by those bytes (4 heads on 1 kv head):
 //   head_dim 128:  268 MB (2048 tokens in blocks of 8, 16 blocks of keys) 21.5 | 29.9, 1070 MB (8192 tokens) 74.6 | 44.8
 //   head_dim 256:  136 MB (128 tokens behind 4096 keys) 21.4 | 25.0, 537 MB (2048 tokens in blocks of 8) 41.6 | 39.0
 //   head_dim 512:   68 MB (32 tokens behind 4096 keys) 27.9 | 29.8, 136 MB (64 tokens) 34.7 | 30.0, one group of 16 rows
 //   of many, 4300 MB: 519 | 440
-static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int most, bool wide, bool joined) {
+static RowsPlan plan_rows(int64_t rows, int64_t count, double live, double all, int64_t tiles, int D, double values, int most, bool wide, bool joined) {
     RowsPlan p;
     p.nw = rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
     // two row groups where four would not give every CU a workgroup even in shares (head_dim 512, 64 tokens behind 4096 keys:
@@ -938,8 +951,15 @@ static RowsPlan plan_rows(int64_t rows, int64_t count, int64_t tiles, int D, int
     if (!wide || few_bytes(rows, count, tiles, D) <= (D < 512 ? 400e6 : 100e6) || (rows <= 16 && D < 512)) p.nw = 0;
     const int R = p.nw ? 32 * p.nw : 16;
     p.tiles = (rows + R - 1) / R;
-    // k_keys_few fills a CU's LDS from head_dim 256 on
-    p.parts = key_shares(p.tiles * count, tiles, p.nw || D < 256 ? 2 : 1, p.nw ? 8 : 4, most);
+    const double groups = std::min((double)p.tiles * live, std::max(live, all / R + 0.5 * live));
+    const double ctx_us = values * 8. / 4e6;  // 4 TB/s
+    if (p.nw) {
+        // workgroups a CU: one at head_dim 512 (LDS), four of two groups at 128 and below; 3.2 TFLOP/s a CU
+        const int each = D == 512 ? 1 : p.nw == 2 && D <= 128 ? 4 : 2;
+        p.parts = key_shares(groups, tiles, each * num_cus(), (double)R * each * D * 128 / 3.2e6, ctx_us, joined, 8, most);
+    } else {
+        p.parts = key_shares(groups, tiles, num_cus(), D * 128 / 40e3, ctx_us, joined, 4, most);  // 40 GB/s a CU
+    }
     // up to six tiles a wave, one workgroup's walk is shorter than a second launch to join shares (one token of 3 heads over
     // 531 keys of 256, us a call: 12.9 | 16.1 in four shares), unless there is one anyway (`joined`)
     if (!p.nw && tiles <= 24 && !joined) p.parts = 1;
@@ -959,18 +979,21 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
     // follows the rows' contexts. us a call, each | shared: head_dim 256, 64 sequences of 1 token of 4 heads behind 2048 keys
     // 19.2 | 21.3, 4096 25.4 | 23.7, 16384 62.6 | 33.3; of 8 tokens 2048 27.1 | 36.8, 8192 62.7 | 55.2.
     p.apart = B > 1 && P > 0 && rows <= 64 && few_bytes(rows, (int64_t)B * KV, pre_tiles, D) > 200e6 + 1400.0 * Mq * H * D;
-    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, pre_tiles, D, kMaxKeyParts / 2, wide_takes(pre), true);
-    p.rows = plan_rows(rows, (int64_t)B * KV, own_tiles + (p.apart ? 0 : pre_tiles), D, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts,
+    const double all = (double)Mq * H, values = all * D;
+    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, KV, all, pre_tiles, D, values, kMaxKeyParts / 2, wide_takes(pre), true);
+    p.rows = plan_rows(rows, (int64_t)B * KV, (double)B * KV, all, own_tiles + (p.apart ? 0 : pre_tiles), D, values, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts,
                        wide_takes(own) && (p.apart || wide_takes(pre)), p.apart);
     if (needs_copy(pre)) p.pad_pre = pad_bytes(P, KV, D);
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
 }
 
-static KeysPlan plan_blocks(const KeySet &own, int B, int max_q, int H, int KV, int D, int q_block, int n_sel) {
+static KeysPlan plan_blocks(int Mq, const KeySet &own, int B, int max_q, int H, int KV, int D, int q_block, int n_sel) {
     KeysPlan p;
     const int64_t NQ = ((int64_t)max_q + q_block - 1) / q_block;
-    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, 2 * (int64_t)n_sel, D, kMaxKeyParts, wide_takes(own), false);
+    const double live = KV * std::min((double)NQ * B, std::max((double)B, (double)Mq / q_block + 0.5 * B));
+    p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, live, INFINITY, 2 * (int64_t)n_sel, D, (double)Mq * H * D, kMaxKeyParts,
+                       wide_takes(own), false);
     p.rows.tiles *= NQ;
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
@@ -986,8 +1009,8 @@ void keys_route_prefix(int Mq, int Mk, int P, int B, int max_q, int max_k, int H
     plan_out(plan_prefix(Mq, {nullptr, nullptr, 0, (Mk + 7) / 8 * 8, Mk}, {nullptr, nullptr, 0, (P + 7) / 8 * 8, P}, B, max_q, max_k, H, KV, D),
              out);
 }
-void keys_route_blocks(int Mk, int B, int max_q, int H, int KV, int D, int q_block, int n_sel, int *out) {
-    plan_out(plan_blocks({nullptr, nullptr, 0, (Mk + 7) / 8 * 8, Mk}, B, max_q, H, KV, D, q_block, n_sel), out);
+void keys_route_blocks(int Mq, int Mk, int B, int max_q, int H, int KV, int D, int q_block, int n_sel, int *out) {
+    plan_out(plan_blocks(Mq, {nullptr, nullptr, 0, (Mk + 7) / 8 * 8, Mk}, B, max_q, H, KV, D, q_block, n_sel), out);
 }
 
 static size_t part_bytes(const KeysPlan &p, int Mq, int H, int D) {
@@ -1163,7 +1186,7 @@ extern "C" size_t e2mi_attention_blocks_workspace_bytes(int Mq, int Mk, int64_t 
                                                         int n_sel) {
     if (!sizes_fit(Mq, B, max_q, 0, H, KV, D) || Mk < 0 || q_block <= 0 || n_sel <= 0 || n_sel > kMaxSelect || !Mq || !B || !max_q)
         return 0;
-    return workspace_of(plan_blocks({nullptr, nullptr, 0, ldv, Mk}, B, max_q, H, KV, D, q_block, n_sel), Mq, H, D);
+    return workspace_of(plan_blocks(Mq, {nullptr, nullptr, 0, ldv, Mk}, B, max_q, H, KV, D, q_block, n_sel), Mq, H, D);
 }
 
 extern "C" int e2mi_attention_blocks(e2mi_stream stream, int dtype, const uint16_t *q, int64_t ldq, int Mq, const uint16_t *k,
@@ -1188,7 +1211,7 @@ extern "C" int e2mi_attention_blocks(e2mi_stream stream, int dtype, const uint16
     }
     if (!Mq || !B || !max_q) return 0;
     a.NQ = (int)(((int64_t)max_q + q_block - 1) / q_block);
-    const KeysPlan p = plan_blocks(a.own, B, max_q, H, KV, D, q_block, n_sel);
+    const KeysPlan p = plan_blocks(Mq, a.own, B, max_q, H, KV, D, q_block, n_sel);
     if (check_workspace("attention_blocks", workspace_of(p, Mq, H, D), workspace, workspace_bytes)) return -1;
     return run_keys((hipStream_t)stream, dtype, D, a, p, workspace);
 }

@@ -134,6 +134,6 @@ def route_blocks(c, q_block, n_sel):
     import ctypes as C
     import e2mi
     out = (C.c_int * 6)()
-    e2mi.load()._ZN4e2mi17keys_route_blocksEiiiiiiiiPi(c["k"].shape[0], len(c["q_lens"]), c["max_q"], c["H"], c["KV"], c["D"], q_block,
+    e2mi.load()._ZN4e2mi17keys_route_blocksEiiiiiiiiiPi(c["Mq"], c["k"].shape[0], len(c["q_lens"]), c["max_q"], c["H"], c["KV"], c["D"], q_block,
                                                        n_sel, out)
     return list(out)

@@ -17,7 +17,20 @@ def prefix(Mq, Mk, P, B, max_q, max_k, H, KV, D):
 
 
 def blocks(Mk, B, max_q, H, KV, D, q_block, n_sel):
-    return _plan("_ZN4e2mi17keys_route_blocksEiiiiiiiiPi", Mk, B, max_q, H, KV, D, q_block, n_sel)
+    return _plan("_ZN4e2mi17keys_route_blocksEiiiiiiiiiPi", B * max_q, Mk, B, max_q, H, KV, D, q_block, n_sel)
+
+
+def test_shares_fill_rounds():
+    """Shares by what a call takes: a round of workgroups that is begun is paid for."""
+    assert prefix(1500, 1500, 4096, 1, 1500, 1500, 4, 1, 512)[3:5] == [4, 5]     # 47 row tiles: 235 workgroups, one a CU
+    assert prefix(40, 40 * 8192, 8, 40, 1, 8192, 8, 4, 256)[3:5] == [0, 3]       # 160: 480, two rounds
+    assert prefix(1, 0, 531, 1, 1, 0, 3, 1, 256)[3:5] == [0, 1]                  # a short walk in one launch
+    assert prefix(1, 0, 8192, 1, 1, 0, 4, 1, 256)[4] >= 32
+    for D in (64, 128, 256, 512):
+        for B in (1, 7, 300):
+            for n in (1, 90, 2000):
+                p = prefix(B * n, B * n, 5000, B, n, n, 4, 2, D)
+                assert 1 <= p[4] and p[2] + p[4] <= 128, p
 
 
 # (Mq, Mk, P, B, max_q, max_k, H, KV, D) -> apart, the prefix's nw, own nw
