@@ -148,8 +148,9 @@ __device__ inline bool start_walk(const KeysArgs &a, int kvh, int b, int tile, i
         if (a.mode == kOwnRows && far > 0) n_own = (far + 31) / 32;
     }
     const int n = w.n_pre + n_own;
-    w.t0 = (int)((int64_t)n * part / a.parts);
-    w.t1 = (int)((int64_t)n * (part + 1) / a.parts);
+    const int each = n / a.parts, rest = n - each * a.parts;
+    w.t0 = part * each + min(part, rest);
+    w.t1 = w.t0 + each + (part < rest);
     return true;
 }
 
@@ -229,6 +230,9 @@ __device__ inline uint32_t here(uint32_t x) {
     return x;
 }
 
+// K and V^T fragments are read this many MFMAs ahead of their use
+constexpr int kFewAhead = 8;
+
 template <class T, int D>
 __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
     typedef typename Half8<T>::type V8;
@@ -238,6 +242,8 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
     constexpr int RPI = 512 / D, LPR = D / 8, NL = D / 16;  // K rows a load fetches, lanes per K row, loads of a tile
     extern __shared__ __align__(16) unsigned char few_smem[];  // the waves' tiles, then the list (kSelected)
     __shared__ float s_m[WV][16], s_l[WV][16];
+    __shared__ float s_f[16][WV];              // what a wave's context counts for
+    __shared__ int64_t s_row[16], s_ctx[16];  // where the rows lie in [Mq][H], in ctx
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -271,13 +277,6 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
         for (int j = 0; j < NL; j++, base = here(base + 16 * (uint64_t)ldB))
             dma16_nc(rsrc_words((const void *)base, 0x7fffffffu), lds0 + (uint32_t)(L::kTile + j * 1024), vo, 0);
     };
-    int t = k.t0 + w;
-    KeyTile now = {}, next = {};
-    if (t < k.t1) {
-        now = key_tile(a, k, list, t);
-        load_k(now);
-        load_v(now);
-    }
     int last;  // own keys this lane's row sees
     V8 qf[NQ];
     {
@@ -286,6 +285,14 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
         const uint16_t *qp = a.q + ((int64_t)k.qs + tok) * a.ldq + (int64_t)h * D + 8 * g;
 #pragma unroll
         for (int s = 0; s < NQ; s++) qf[s] = *(const V8 *)(qp + 32 * s);
+        if (tid < 16) s_row[tid] = ((int64_t)k.qs + tok) * a.H + h, s_ctx[tid] = ((int64_t)k.qs + tok) * a.ldc + (int64_t)h * D;
+    }
+    int t = k.t0 + w;
+    KeyTile now = {}, next = {};
+    if (t < k.t1) {
+        now = key_tile(a, k, list, t);
+        load_k(now);
+        load_v(now);
     }
     f4v o[NO];
 #pragma unroll
@@ -296,18 +303,25 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
 #pragma unroll
     for (int u = 0; u < 2; u++) krd[u] = (uint32_t)((8 * (c >> 2) + 4 * u + (c & 3)) * 2 * D);
     const uint32_t vrd = (uint32_t)(c * 64 + ((g ^ ((c >> 2) & 3)) << 4));
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // everything so far; inside the loop the compiler must find nothing to wait for
 
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // everything so far; inside the loop the compiler must find nothing to wait for
     for (; t < k.t1; t += WV, now = next) {
         const bool more = t + WV < k.t1;
         // the tile's K has landed (V^T was requested after it)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
         f4v st[2] = {};
+        {
+            auto kfrag = [&](int x) { return *(const V8 *)(sk + krd[x & 1] + (((4 * (x >> 1) + g) ^ fc) << 4)); };
+            V8 kr[kFewAhead];
 #pragma unroll
-        for (int s = 0; s < NQ; s++)
+            for (int x = 0; x < kFewAhead && x < 2 * NQ; x++) kr[x] = kfrag(x);
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-                st[u] = mma16<T>(*(const V8 *)(sk + krd[u] + (((4 * s + g) ^ fc) << 4)), qf[s], st[u]);
+            for (int x = 0; x < 2 * NQ; x++) {
+                st[x & 1] = mma16<T>(kr[x % kFewAhead], qf[x >> 1], st[x & 1]);
+                if (x + kFewAhead < 2 * NQ) kr[x % kFewAhead] = kfrag(x + kFewAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
         if (more) {
             next = key_tile(a, k, list, t + WV);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its reads are done
@@ -355,15 +369,24 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
                 for (int e = 0; e < 4; e++) x[e] &= have >= 2 * e + 2 ? 0xffffffffu : have == 2 * e + 1 ? 0xffffu : 0u;
             }
         }
+        {
+            V8 vr[kFewAhead];
 #pragma unroll
-        for (int i = 0; i < NO; i++) o[i] = mma16<T>(*(const V8 *)(sv + vrd + i * 1024), pb, o[i]);
+            for (int i = 0; i < kFewAhead && i < NO; i++) vr[i] = *(const V8 *)(sv + vrd + i * 1024);
+#pragma unroll
+            for (int i = 0; i < NO; i++) {
+                o[i] = mma16<T>(vr[i % kFewAhead], pb, o[i]);
+                if (i + kFewAhead < NO) vr[i % kFewAhead] = *(const V8 *)(sv + vrd + (i + kFewAhead) * 1024);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             load_v(next);
         }
     }
 
-    // join the waves: contexts as they are, with their maxima and sums; a quad of dims a thread
+    // join the waves: contexts as they are, what each counts for by 16 threads, then a quad of dims a thread
     float lsum = lrun + xor_lane<16>(lrun);
     lsum += xor_lane<32>(lsum);
     if (g == 0) s_m[w][c] = mrun, s_l[w][c] = lsum;
@@ -374,42 +397,50 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
 #pragma unroll
         for (int i = 0; i < NO; i++) *(f4v *)(y + 16 * i) = o[i];
     }
-    __syncthreads();
-#pragma unroll 1
-    for (int at = tid; at < 4 * D; at += 64 * WV) {
-        const int row = at / (D / 4), d = at % (D / 4) * 4, r = k.r0 + row;
-        float mall = s_m[0][row];
+    if (tid < 16) {
+        float mall = s_m[0][tid], f[WV], sum = 0.f;
 #pragma unroll
-        for (int x = 1; x < WV; x++) mall = fmaxf(mall, s_m[x][row]);
-        f4v v = {};
-        float sum = 0.f;
+        for (int x = 1; x < WV; x++) mall = fmaxf(mall, s_m[x][tid]);
 #pragma unroll
         for (int x = 0; x < WV; x++) {
-            const float mx = s_m[x][row], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mall);
-            v += *(const f4v *)(ctx + (x * 16 + row) * PITCH + d) * f;
-            sum += s_l[x][row] * f;
+            const float mx = s_m[x][tid];
+            f[x] = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mall);
+            sum += s_l[x][tid] * f[x];
         }
-        if (sum != sum) v = (f4v)NAN;
-        const bool live = r < k.rows;
-        const int rc = live ? r : k.rows - 1, h = k.kvh * a.G + rc % a.G;
-        const int64_t m = (int64_t)k.qs + k.tok0 + rc / a.G;
+        // a NaN sum (NaN rows) takes the whole row with it
+        const float scale = sum != sum ? NAN : a.part_o ? 1.f : sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+#pragma unroll
+        for (int x = 0; x < WV; x++) s_f[tid][x] = f[x] * scale;
         if (a.part_o) {
-            const int64_t to = ((int64_t)(a.part0 + k.part) * a.Mq + m) * a.H + h;
-            if (live && d == 0) write_share(a, to, mall, sum);
-            if (live && sum != 0.f) *(f4v *)(a.part_o + to * D + d) = v;
+            s_row[tid] += (int64_t)(a.part0 + k.part) * a.Mq * a.H;
+            if (k.r0 + tid < k.rows) write_share(a, s_row[tid], mall, sum);
+            s_l[0][tid] = sum;
+        }
+    }
+    __syncthreads();
+    constexpr int EACH = 4 * D / (64 * WV);  // quads a thread
+#pragma unroll 4
+    for (int i = 0; i < EACH; i++) {
+        const int at = tid + 64 * WV * i, row = at / (D / 4), d = at % (D / 4) * 4;
+        f4v v = {};
+#pragma unroll
+        for (int x = 0; x < WV; x++) v += *(const f4v *)(ctx + (x * 16 + row) * PITCH + d) * s_f[row][x];
+        const bool live = k.r0 + row < k.rows;
+        const int64_t mh = s_row[row];
+        if (a.part_o) {
+            if (live && s_l[0][row] != 0.f) *(f4v *)(a.part_o + mh * D + d) = v;
             continue;
         }
-        v *= sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
         if (a.ctx && live) {
             const T4 y = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-            *(T4 *)((T *)a.ctx + m * a.ldc + (int64_t)h * D + d) = y;
+            *(T4 *)((T *)a.ctx + s_ctx[row] + d) = y;
         }
         if constexpr (D % 128 == 0) {
             if (a.cq) {  // 128 dims: 32 lanes
                 const QScale q = qscale(group_max<32>(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))));
                 if (live) {
-                    *(uint32_t *)(a.cq + (m * a.H + h) * D + d) = pack4_magic(v[0], v[1], v[2], v[3], q.inv);
-                    if (d % 128 == 0) a.cs[(m * a.H + h) * (D / 128) + d / 128] = q.sc;
+                    *(uint32_t *)(a.cq + mh * D + d) = pack4_magic(v[0], v[1], v[2], v[3], q.inv);
+                    if (d % 128 == 0) a.cs[mh * (D / 128) + d / 128] = q.sc;
                 }
             }
         }
