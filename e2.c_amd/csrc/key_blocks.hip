@@ -128,12 +128,24 @@ __device__ inline int byte_lanes_negative(uint32_t x) {  // 0xff in every negati
     return (int)((m << 8) - m);
 }
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+template <int D>
+struct ScoreTile {
+    static constexpr int kTile = 64 * D;               // bytes of 32 blocks' bounds
+    static constexpr int NB = D <= 256 ? 3 : 2;        // buffers (head_dim 512: two, so that two workgroups fit a CU)
+    static constexpr int kScale = NB * kTile;          // the tiles' scales, 256 bytes each
+    static constexpr int kBest = kScale + NB * 256;
+};
+// The scales of a tile's blocks, a lane's 4 bytes each (past the buffer's end: zeros).
+__device__ inline void dma4(v4u r, uint32_t lds, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r) : "memory");
+}
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int shares, int groups) {
-    constexpr int NS = D / 32, TILE = 64 * D, RPI = 512 / D, LPR = D / 8, NLW = D / 64;
-    extern __shared__ __align__(16) unsigned char sc_smem[];  // two tiles of bounds, then the maxima (span > 1)
-    __shared__ int s_last[128];
-    __shared__ float s_scale[128];
+    using L = ScoreTile<D>;
+    constexpr int NS = D / 32, RPI = 512 / D, LPR = D / 8, NLW = D / 64;
+    extern __shared__ __align__(16) unsigned char sc_smem[];  // tiles of bounds, their scales, then the maxima (span > 1)
+    __shared__ __align__(16) int s_last[128];
+    __shared__ __align__(16) float s_scale[128];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wu = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = xcd_swizzle(blockIdx.x, gridDim.x);
@@ -151,9 +163,9 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
     if ((int64_t)qb0 * a.q_block >= nq) return;
     const int nk = max(0, min(a.k_len[b], a.max_k));
     const int nb = (nk + kKeyBlock - 1) / kKeyBlock, all = (nb + 31) / 32;  // blocks, tiles of them
-    const int t0 = (int)((int64_t)all * share / shares), t1 = (int)((int64_t)all * (share + 1) / shares);
+    const int t0 = (int)((unsigned)(all * share) / (unsigned)shares), t1 = (int)((unsigned)(all * (share + 1)) / (unsigned)shares);  // all, shares <= 1024
     if (t0 >= t1) return;
-    uint32_t *s_best = (uint32_t *)(sc_smem + 2 * TILE);  // [wg_blocks][32 (t1 - t0)]: order keys, 0: none
+    uint32_t *s_best = (uint32_t *)(sc_smem + L::kBest);  // [wg_blocks][32 (t1 - t0)]: order keys, 0: none
     const int width = 32 * (t1 - t0);
     if (span > 1)
         for (int i = tid; i < width * wg_blocks; i += 256) s_best[i] = 0;
@@ -161,17 +173,24 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_void *)sc_smem);
     const int lr = lane / LPR, lc = lane % LPR;
     const uint32_t ldb = (uint32_t)a.KV * 2 * D;
-    auto load = [&](int t, int buf) {  // bounds of blocks 32 t .. + 31; those past the last read as zero
-        const int n0 = 32 * t, have = min(32, nb - n0);
+    auto load = [&](int t) {  // bounds of blocks 32 t .. + 31; those past the last read as zero
+        const int n0 = 32 * t, have = min(32, nb - n0), buf = (t - t0) % L::NB;
+        if (span == 1 && wu == 0)
+            dma4(rsrc_words(a.kscale + ((int64_t)b * a.NB + n0) * a.KV + kvh, (uint32_t)((have - 1) * a.KV + 1) * 4),
+                 __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(L::kScale + buf * 256)), lane < 32 ? (uint32_t)(lane * a.KV) * 4 : 0x80000000u);
         const v4u rs = rsrc_words(a.bounds + (((int64_t)b * a.NB + n0) * a.KV + kvh) * (2 * D), (uint32_t)(have - 1) * ldb + 2 * D);
 #pragma unroll
         for (int j = 0; j < NLW; j++) {
             const int r = RPI * (NLW * wu + j);
-            dma16(rs, __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(buf * TILE + r * 2 * D)),
+            dma16(rs, __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(buf * L::kTile + r * 2 * D)),
                   (uint32_t)(r + lr) * ldb + (uint32_t)((lc ^ ((r + lr) & 7)) << 4), 0);
         }
     };
-    load(t0, 0);  // in flight while the rows are quantized
+    auto start = [&] {
+#pragma unroll 1
+        for (int t = t0; t < min(t0 + L::NB - 1, t1); t++) load(t);
+    };
+    start();  // in flight while the rows are quantized
     const int passes = span > 4 ? (span + 3) / 4 : 1;
     for (int pass = 0; pass < passes; pass++) {
         // this wave's slot: query block `blk` (of the workgroup; span 1: its first), rows from r0 of it
@@ -180,7 +199,9 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
         const bool live = blk < wg_blocks && r0 < R && (int64_t)(qb0 + blk) * a.q_block < nq;
         // quantize: lane (row, half) holds 16 values of every 32
         v4i up[NS], down[NS];
-        {
+        int least = -1, most = -1;  // the last keys that its rows see
+        float sc[16];               // the scales; lane: column (a block), register r: slot 8 (r / 4) + 4 half + r % 4
+        if (live) {
             const int slot = lane & 31, in = span > 1 ? r0 + slot : slot % a.group;
             const int64_t tok = (int64_t)(qb0 + blk + (span > 1 ? 0 : slot / a.group)) * a.q_block + in / a.G;
             const bool row = live && in < R && tok < nq && in / a.G < a.q_block;
@@ -210,35 +231,41 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
                     up[s][e] = (int)(x & ~neg);
                     down[s][e] = (int)(x & neg);
                 }
+            const int seen = !row ? -1 : a.causal ? (int)tok + nk - nq : nk - 1;
             if (half == 0) {
                 s_scale[wu * 32 + slot] = row ? q.sc : NAN;
-                s_last[wu * 32 + slot] = !row ? -1 : a.causal ? (int)tok + nk - nq : nk - 1;
+                s_last[wu * 32 + slot] = seen;
+            }
+            // the first of a wave's slots has a row if any has, and later rows see no less
+            const uint32_t rows = (uint32_t)__ballot(row);
+            least = __builtin_amdgcn_readfirstlane(seen);
+            most = rows ? __builtin_amdgcn_readlane(seen, 31 - __builtin_clz(rows)) : -1;
+            // a wave's own entries only: no barrier
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 x = *(const float4 *)(s_scale + wu * 32 + 8 * i + 4 * half);
+                sc[4 * i] = x.x, sc[4 * i + 1] = x.y, sc[4 * i + 2] = x.z, sc[4 * i + 3] = x.w;
             }
         }
-        // lane: column (a block); register r: slot 8 (r / 4) + 4 half + r % 4. A wave's own entries only: no barrier
-        float sc[16];
-        int least = nk - 1, most = -1;  // the last keys that its rows see
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int slot = wu * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-            sc[r] = s_scale[slot];
-            if (sc[r] == sc[r]) least = min(least, s_last[slot]), most = max(most, s_last[slot]);
-        }
-        least = min(least, __builtin_bit_cast(int, xor_lane<32>(__builtin_bit_cast(float, least))));
-        most = max(most, __builtin_bit_cast(int, xor_lane<32>(__builtin_bit_cast(float, most))));
-
         if (pass) {
             lds_barrier();  // the buffers' last readers are done
-            load(t0, 0);
+            start();
         }
+        // span 1: the slot's query blocks and their scores
+        const int there = live ? min(per, (nq - (qb0 + blk) * a.q_block + a.q_block - 1) / a.q_block) : 0;
+        float *out = a.scores + (((int64_t)b * a.NQ + qb0 + blk) * a.KV + kvh) * a.NB;
+        const int64_t pitch = (int64_t)a.KV * a.NB;
         const uint32_t rd = (uint32_t)((lane & 31) * 2 * D + ((half ^ (lane & 7)) << 4));
         for (int t = t0; t < t1; t++) {
-            const int buf = (t - t0) & 1;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const int buf = (t - t0) % L::NB;
+            // this wave's loads of the tile have landed (NB 3: those of the next may be on their way); the barrier makes every
+            // wave's visible and ends every wave's reads of the buffer that the next load fills
+            if (L::NB > 2 && t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NLW) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (t + 1 < t1) load(t + 1, buf ^ 1);
+            if (t + L::NB - 1 < t1) load(t + L::NB - 1);
             if (!live || (int64_t)32 * t * kKeyBlock > most) continue;
-            const unsigned char *sb = sc_smem + buf * TILE;
+            const unsigned char *sb = sc_smem + buf * L::kTile;
             auto frag = [&](int s) { return *(const v4i *)(sb + (rd ^ (uint32_t)((s & 3) << 5)) + (s >> 2) * 128); };
             v16i acc = {};
             v4i f[4];
@@ -272,10 +299,9 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
                 if (half == 0 && v == v) atomicMax(s_best + blk * width + n - 32 * t0, order_key(v));
                 continue;
             }
-            const float ks = n < nb ? a.kscale[((int64_t)b * a.NB + n) * a.KV + kvh] : 0.f;
+            const float ks = *(const float *)(sc_smem + L::kScale + buf * 256 + 4 * (lane & 31));
             auto put = [&](int i, float v) {
-                if (n < nb && (int64_t)(qb0 + blk + i) * a.q_block < nq)
-                    a.scores[(((int64_t)b * a.NQ + qb0 + blk + i) * a.KV + kvh) * a.NB + n] = __fmul_rn(v, ks);
+                if (n < nb && i < there) out[i * pitch + n] = __fmul_rn(v, ks);
             };
             if (a.group == 4) {
 #pragma unroll
@@ -453,7 +479,7 @@ static int launch_scores(hipStream_t st, const SelectArgs &a, int B) {
         set_error("block_select: too many rows for a launch");
         return -1;
     }
-    const size_t lds = 128 * D + (span > 1 ? (size_t)((tiles + shares - 1) / shares) * 128 * wg_blocks : 0);
+    const size_t lds = ScoreTile<D>::kBest + (span > 1 ? (size_t)((tiles + shares - 1) / shares) * 128 * wg_blocks : 0);
     static LdsAllowed allowed;
     if (allow_lds((const void *)k_block_scores<T, D>, (int)lds, allowed)) return -1;
     hipLaunchKernelGGL((k_block_scores<T, D>), dim3((unsigned)grid), dim3(256), lds, st, a, (int)shares, (int)groups);
