@@ -274,8 +274,8 @@ def set_gemm_fold(mode: str) -> str:
 def _stream(stream):
     if stream is not None:
         return stream.cuda_stream
-    import torch
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    current, device = _torch()[1:3]
+    return current(device())
 
 
 def _p(t):
@@ -760,32 +760,36 @@ def gather_ids(ids, rowmap, stream=None):
 # Single tokens are calls of a few microseconds: each operand is looked at once, and sizes that follow from sizes are
 # kept (functools.lru_cache).
 @functools.lru_cache(maxsize=None)
-def _dtype_codes():
+@functools.lru_cache(maxsize=None)
+def _torch():
+    """What every call below takes of torch, looked up once: ({type: the library's code}, the current raw stream, the current
+    device, int32, uint8, empty)."""
     import torch
-    return {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+    return ({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}, torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice,
+            torch.int32, torch.uint8, torch.empty)
 
 
 def _kind(name, t):
     """The library's code of a tensor's type, and its device, which has to be the current one."""
-    import torch
-    kind, dev = _dtype_codes().get(t.dtype), t.get_device()
+    codes, _, device, _, _, _ = _torch()
+    kind, dev = codes.get(t.dtype), t.get_device()
     if kind is None:
         raise E2MIError(f"{name}: needs f16, bf16 or f32 rows, got {t.dtype}")
-    if dev < 0 or dev != torch._C._cuda_getDevice():
+    if dev < 0 or dev != device():
         raise E2MIError(f"{name}: needs tensors on the current device, got one on {t.device}")
     return kind, dev
 
 
 def _rows(name, t, rows, width, dtype, dev):
     """Address and pitch of a tensor [rows, width] with contiguous rows."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or shape[0] != rows or shape[1] != width:
-        raise E2MIError(f"{name}: needs rows [{rows}, {width}], got {tuple(shape)}")
+    if t.shape != (rows, width):
+        raise E2MIError(f"{name}: needs rows [{rows}, {width}], got {tuple(t.shape)}")
     if t.dtype is not dtype or t.get_device() != dev:
         raise E2MIError(f"{name}: needs {dtype} tensors on device {dev}, got {t.dtype} on {t.device}")
-    if stride[1] != 1 and width > 1:
+    pitch, step = t.stride()
+    if step != 1 and width > 1:
         raise E2MIError(f"{name}: needs rows of contiguous values")
-    return t.data_ptr(), stride[0] if rows > 1 else max(stride[0], width)
+    return t.data_ptr(), pitch if rows > 1 or pitch > width else width
 
 
 def _head_dim(name, t, H, KV):
@@ -797,8 +801,7 @@ def _head_dim(name, t, H, KV):
 
 def _indices(name, t, n, dev):
     """Address of a contiguous int32 device array of at least n entries."""
-    import torch
-    if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous() or t.numel() < n:
+    if t.dtype is not _torch()[3] or t.get_device() != dev or not t.is_contiguous() or t.numel() < n:
         raise E2MIError(f"{name}: needs contiguous int32 arrays of at least {n} values on device {dev}")
     return t.data_ptr()
 
@@ -887,13 +890,13 @@ def _keys(name, k, vt, KV, D, dtype, dev):
 def _context(name, q, M, width, ctx, quant, stream, dev):
     """The outputs (ctx, its address and pitch, the pair, its addresses): ctx given or made (zeros, so that rows outside
     every sequence are defined), or the quantized pair."""
-    import torch
     if not quant:
         if ctx is None:
             ctx = _new(stream, q.new_zeros, (M, width))
         return ctx, *_rows(name, ctx, M, width, q.dtype, dev), None, None, None
     if ctx is not None:
         raise E2MIError(f"{name}: either ctx or the quantized pair")
+    import torch
     cq = _new(stream, torch.zeros, (M, width), dtype=torch.int8, device=q.device)
     cs = _new(stream, torch.zeros, (M, width // 128), dtype=torch.float32, device=q.device)
     return None, None, 0, (cq, cs), cq.data_ptr(), cs.data_ptr()
@@ -904,8 +907,8 @@ def _workspace(name, need, workspace, like, stream, dev):
     if workspace is None:
         if not need:
             return None, None, 0
-        import torch
-        workspace = _new(stream, torch.empty, need, dtype=torch.uint8, device=like.device)
+        _, _, _, _, uint8, empty = _torch()
+        workspace = empty(need, dtype=uint8, device=like.device) if stream is None else _new(stream, empty, need, dtype=uint8, device=like.device)
         return workspace, workspace.data_ptr(), need
     if workspace.get_device() != dev or not workspace.is_contiguous():
         raise E2MIError(f"{name}: needs a contiguous workspace on device {dev}")
