@@ -344,7 +344,7 @@ __device__ inline uint32_t wave_max(uint32_t v) {
 // The n_sel largest: the n_sel-th largest key by bisection of the bits in which the keys differ (counts by ballots
 // over keys held in registers), ended as soon as a count is n_sel; then everything above it and the first of its equals,
 // in block order. W waves a list, RPL keys a lane: key 64 (w RPL + j) + lane is register j of wave w. Bound by the
-// latency of its counts: 16 lists of 1024 blocks 6.7 us (four waves a list), 4096 lists 17.
+// latency of its counts: 16 lists of 1024 blocks 6.7 us (four waves a list), 1024 of them 16.6.
 template <int W, int RPL>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_block_top(SelectArgs a, int64_t lists) {
     constexpr int WG = W > 4 ? W : 4;  // waves a workgroup
