@@ -44,22 +44,44 @@ struct KeysArgs {
 
 // A sequence's row range, cut to the call's limit; false for none, or for one outside the rows given (read
 // as empty: an access never leaves the tensors, whatever the device arrays hold).
-__device__ inline bool row_range(const int32_t *start, const int32_t *len, int b, int most, int rows, int &s, int &n) {
-    s = start[b];
-    n = min(len[b], most);
+__device__ inline bool row_range(int start, int len, int most, int rows, int &s, int &n) {
+    s = start;
+    n = min(len, most);
     if (n <= 0 || s < 0 || (int64_t)s + n > rows) {
         s = n = 0;
         return false;
     }
     return true;
 }
+__device__ inline bool row_range(const int32_t *start, const int32_t *len, int b, int most, int rows, int &s, int &n) {
+    return row_range(start[b], len[b], most, rows, s, n);
+}
 // The same of keys, whose starts are multiples of 8 (V^T is read in 16-byte chunks).
-__device__ inline bool key_range(const int32_t *start, const int32_t *len, int b, int most, int rows, int &s, int &n) {
-    if (!row_range(start, len, b, most, rows, s, n) || (s & 7)) {
+__device__ inline bool key_range(int start, int len, int most, int rows, int &s, int &n) {
+    if (!row_range(start, len, most, rows, s, n) || (s & 7)) {
         s = n = 0;
         return false;
     }
     return true;
+}
+
+// Loads that are wanted at once: without this the compiler moves each to its first use, behind the branches before it, and
+// their latencies (0.5 us and more of a cold line) add up.
+__device__ inline void wanted(int &x) {
+    x = __builtin_amdgcn_readfirstlane(x);
+    asm volatile("" : "+s"(x));
+}
+template <class... I>
+__device__ inline void together(I &...x) {
+    (wanted(x), ...);
+}
+// The same for a kernel's arguments, a value of each of their lines.
+template <class A>
+__device__ inline void touch(const A &a) {
+    const int *p = (const int *)&a;
+    constexpr int n = sizeof(A) / 64;
+    static_assert(n <= 5, "lines of arguments");
+    asm volatile("" ::"s"(p[0]), "s"(p[n > 1 ? 16 : 0]), "s"(p[n > 2 ? 32 : 0]), "s"(p[n > 3 ? 48 : 0]), "s"(p[n > 4 ? 64 : 0]));
 }
 
 // Allows a kernel `bytes` of dynamic LDS, once a device for its largest need so far (`allowed`: a static of the caller's,

@@ -123,8 +123,10 @@ __device__ inline bool start_walk(const KeysArgs &a, int kvh, int b, int tile, i
     }
     w.qs = 0, w.nq = a.Mq, w.ks = 0, w.nk = 0;
     if (a.mode != kAllRows) {
-        if (!row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, w.qs, w.nq)) return false;
-        if (a.own.rows) key_range(a.k_start, a.k_len, b, a.max_k, a.own.rows, w.ks, w.nk);
+        int q0 = a.q_start[b], nq = a.q_len[b], k0 = a.k_start[b], nk = a.k_len[b];
+        together(q0, nq, k0, nk);
+        if (!row_range(q0, nq, a.max_q, a.Mq, w.qs, w.nq)) return false;
+        if (a.own.rows) key_range(k0, nk, a.max_k, a.own.rows, w.ks, w.nk);
     }
     int ntok = w.nq;
     w.tok0 = 0, w.r0 = tile * R;
@@ -250,6 +252,7 @@ __global__ __launch_bounds__(64 * FewTile<D>::WV) void k_keys_few(KeysArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int *list = (int *)(few_smem + L::kBytes);
+    touch(a);
     Walk k;
     if (!start_walk<16>(a, blockIdx.y, blockIdx.z, (int)(blockIdx.x / (unsigned)a.parts), (int)(blockIdx.x % (unsigned)a.parts), list,
                         &s_count, k))

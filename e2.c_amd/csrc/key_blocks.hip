@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void k_block_bounds(BoundsArgs a) {
     __shared__ float s_amax[4];
     const int tid = threadIdx.x, n = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     int ks, nk;
-    if (!key_range(a.k_start, a.k_len, b, a.max_k, a.Mk, ks, nk) || n * kKeyBlock >= nk) return;
+    if (!key_range(a.k_start[b], a.k_len[b], a.max_k, a.Mk, ks, nk) || n * kKeyBlock >= nk) return;
     const int keys = min(kKeyBlock, nk - n * kKeyBlock);
     const int ch = tid % CH, rg = tid / CH;
     const uint16_t *kp = a.k + ((int64_t)ks + n * kKeyBlock) * a.ldk + (int64_t)kvh * D + ch * 8;
@@ -150,6 +150,7 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
     __shared__ __align__(16) float s_scale[128];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wu = __builtin_amdgcn_readfirstlane(tid >> 6);
+    touch(a);
     int id = xcd_swizzle(blockIdx.x, gridDim.x);
     const int share = id % shares;
     id /= shares;
@@ -160,10 +161,11 @@ __global__ __launch_bounds__(256, 2) void k_block_scores(SelectArgs a, int share
     const int per = 32 / a.group;                            // query blocks of a slot (span 1)
     const int wg_blocks = span > 4 ? 1 : span > 1 ? 4 / span : 4 * per;  // query blocks of this workgroup
     const int qb0 = at * wg_blocks;
-    int qs, nq;
-    if (!row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, qs, nq)) return;
+    int qs, nq, q0 = a.q_start[b], ql = a.q_len[b], kl = a.k_len[b];
+    together(q0, ql, kl);
+    if (!row_range(q0, ql, a.max_q, a.Mq, qs, nq)) return;
     if ((int64_t)qb0 * a.q_block >= nq) return;
-    const int nk = max(0, min(a.k_len[b], a.max_k));
+    const int nk = max(0, min(kl, a.max_k));
     const int nb = (nk + kKeyBlock - 1) / kKeyBlock, all = (nb + 31) / 32;  // blocks, tiles of them
     const int t0 = (int)((unsigned)(all * share) / (unsigned)shares), t1 = (int)((unsigned)(all * (share + 1)) / (unsigned)shares);  // all, shares <= 1024
     if (t0 >= t1) return;
@@ -357,8 +359,10 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_block_top(SelectArgs a
     const int qb = (int)(id / a.KV % a.NQ), b = (int)(id / a.KV / a.NQ);
     int32_t *out = a.sel + id * a.n_sel;
     int qs, nq;
-    const bool has = row_range(a.q_start, a.q_len, b, a.max_q, a.Mq, qs, nq) && (int64_t)qb * a.q_block < nq;
-    const int nk = max(0, min(a.k_len[b], a.max_k));
+    int q0 = a.q_start[b], ql = a.q_len[b], kl = a.k_len[b];
+    together(q0, ql, kl);  // a list is a wave's at least
+    const bool has = row_range(q0, ql, a.max_q, a.Mq, qs, nq) && (int64_t)qb * a.q_block < nq;
+    const int nk = max(0, min(kl, a.max_k));
     const int t0 = qb * a.q_block, t1 = min(t0 + a.q_block, nq) - 1;
     const int far = !has ? -1 : a.causal ? min(t1 + nk - nq, nk - 1) : nk - 1;  // last key any row sees
     const int p0 = t0 + nk - nq, p1 = t1 + nk - nq;  // where the block's queries stand among the keys
