@@ -974,20 +974,24 @@ static bool wide_takes(const KeySet &s) { return !s.rows || s.ldv < (1 << 23); }
 static double few_bytes(int64_t rows, int64_t count, int64_t tiles, int D) { return (double)((rows + 15) / 16 * count) * tiles * 128 * D; }
 
 // `count` groups (sequences, query blocks; times kv heads) of at most `rows` rows over `tiles` key tiles. The lengths are on
-// the device; the host's guess is that `live` of the groups have rows, `all` together. values: of the context. Which kernel: few rows are
-// faster where the keys that its tiles ask for again come from L2 in about the time of the launch, and a group of 16
-// rows or fewer asks once anyway. us a call, k_keys_few | k_keys_wide, by those bytes (4 heads on 1 kv head):
-//   head_dim 128:  268 MB (2048 tokens in blocks of 8, 16 blocks of keys) 21.5 | 29.9, 1070 MB (8192 tokens) 74.6 | 44.8
-//   head_dim 256:  136 MB (128 tokens behind 4096 keys) 21.4 | 25.0, 537 MB (2048 tokens in blocks of 8) 41.6 | 39.0
-//   head_dim 512:   68 MB (32 tokens behind 4096 keys) 27.9 | 29.8, 136 MB (64 tokens) 34.7 | 30.0, one group of 16 rows
-//   of many, 4300 MB: 519 | 440
+// the device; the host's guess is that `live` of the groups have rows, `all` together. values: of the context. Which kernel:
+// few rows are faster where the keys that its tiles ask for again come from L2 in about the time of the launch, and a
+// group of 16 rows or fewer asks once anyway. us a call, k_keys_few | k_keys_wide, by those bytes (4 heads on 1 kv head unless
+// said; wide's tiles cost more to start the larger head_dim, and at 512 it has four times the rows a key read from LDS):
+//   head_dim  64: 134 MB (2048 tokens in blocks of 8, 16 blocks of keys) 13.9 | 22.6, 268 MB (256 tokens on 2 kv heads
+//                 behind 16384 keys) 39.0 | 27.3
+//   head_dim 128: 277 MB (64 x 16 tokens behind 2048) 23.5 | 28.4, 537 MB (512 tokens behind 8192) 50.8 | 35.9
+//   head_dim 256: 554 MB (64 x 16 tokens behind 2048) 32.4 | 37.0, 1074 MB (256 tokens on 2 behind 16384) 71.9 | 63.5
+//   head_dim 512: 136 MB (64 tokens behind 4096) 27.5 | 30.2, 273 MB (128 tokens) 35.5 | 33.2; 8192 tokens, 16 blocks of keys
+//                 for each 16 rows 342 | 433, for each 24 347 | 222
+static double few_most(int D) { return D == 128 ? 350e6 : D == 256 ? 600e6 : 200e6; }
 static RowsPlan plan_rows(int64_t rows, int64_t count, double live, double all, int64_t tiles, int D, double values, int most, bool wide, bool joined) {
     RowsPlan p;
     p.nw = rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
-    // two row groups where four would not give every CU a workgroup even in shares (head_dim 512, 64 tokens behind 4096 keys:
-    // 30.0 | 38.0 with four)
+    // two row groups where four would not give every CU a workgroup even in shares (head_dim 512, 128 tokens behind 4096 keys:
+    // 33.2 | 38.4 with four)
     if ((rows + 127) / 128 * count * std::min<int64_t>(most, std::max<int64_t>(1, tiles / 8)) < num_cus()) p.nw = 2;
-    if (!wide || few_bytes(rows, count, tiles, D) <= (D < 512 ? 400e6 : 100e6) || (rows <= 16 && D < 512)) p.nw = 0;
+    if (!wide || few_bytes(rows, count, tiles, D) <= few_most(D) || rows <= 16) p.nw = 0;
     const int R = p.nw ? 32 * p.nw : 16;
     p.tiles = (rows + R - 1) / R;
     const double groups = std::min((double)p.tiles * live, std::max(live, all / R + 0.5 * live));

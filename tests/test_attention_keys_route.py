@@ -43,8 +43,8 @@ def test_shares_fill_rounds():
     ((64 * 512, 64 * 512, 2048, 64, 512, 512, 3, 1, 256), 0, None, 4),
     ((64 * 512, 64 * 512, 200000, 64, 512, 512, 3, 1, 256), 0, None, 4),  # long sequences never share a prefix's tiles
     ((128, 0, 4096, 1, 128, 0, 4, 1, 256), 0, None, 0),
-    ((64, 0, 4096, 1, 64, 0, 4, 1, 512), 0, None, 2),
-    ((32, 0, 4096, 1, 32, 0, 4, 1, 512), 0, None, 0),
+    ((128, 0, 4096, 1, 128, 0, 4, 1, 512), 0, None, 2),
+    ((64, 0, 4096, 1, 64, 0, 4, 1, 512), 0, None, 0),
 ])
 def test_prefix(shape, apart, pre, own):
     p = prefix(*shape)
@@ -53,7 +53,7 @@ def test_prefix(shape, apart, pre, own):
 
 
 @pytest.mark.parametrize("shape,nw", [
-    ((8192, 1, 8192, 4, 1, 256, 8, 16), 2), ((8192, 1, 8192, 4, 1, 256, 4, 16), 0), ((8192, 1, 8192, 4, 1, 512, 4, 16), 2),
+    ((8192, 1, 8192, 4, 1, 256, 8, 16), 2), ((8192, 1, 8192, 4, 1, 256, 4, 16), 0), ((8192, 1, 8192, 4, 1, 512, 4, 16), 0), ((8192, 1, 8192, 4, 1, 512, 6, 16), 2),
     ((8192, 1, 2048, 4, 1, 128, 8, 16), 0), ((8192, 1, 8192, 4, 1, 128, 8, 16), 2), ((16384, 1, 16384, 3, 1, 256, 32, 16), 3),
     ((65536, 16, 1, 4, 1, 256, 1, 32), 0), ((16384, 1, 16384, 4, 1, 256, 64, 16), 4),
 ])

@@ -22,9 +22,10 @@ def _lens(seed, n, lo, hi):
 
 PREFIX = [
     # dtype, H, KV, D, q lengths, k lengths (None: the q's), prefix, the plan's nw (own launch)
-    ("float16", 4, 1, 256, _lens(1, 3, 300, 701), None, 333, 4),          # odd prefix: V^T copied
-    ("bfloat16", 3, 1, 256, _lens(2, 120, 9, 21), None, 1024, 2),         # 63 rows: two row groups
-    ("bfloat16", 3, 1, 256, _lens(3, 70, 0, 32), _lens(4, 70, 0, 90), 1100, 3),   # 96 rows, some without any
+    ("float16", 4, 1, 256, _lens(1, 3, 300, 701), None, 1333, 4),         # odd prefix: V^T copied
+    ("bfloat16", 3, 1, 256, _lens(2, 120, 9, 21), None, 2048, 2),         # 63 rows: two row groups
+    ("bfloat16", 3, 1, 256, _lens(3, 70, 0, 32), _lens(4, 70, 0, 90), 2100, 3),   # 96 rows, some without any
+    ("bfloat16", 3, 1, 256, _lens(3, 70, 0, 32), _lens(4, 70, 0, 90), 1100, 0),   # the other kernel, at its largest
     ("float16", 8, 2, 128, _lens(5, 4, 500, 1500), None, 256, 4),
     ("bfloat16", 4, 1, 128, _lens(6, 400, 1, 16), _lens(7, 400, 0, 40), 1000, 2),
     ("float16", 6, 1, 128, _lens(8, 300, 3, 16), None, 1001, 3),
@@ -33,8 +34,8 @@ PREFIX = [
     ("float16", 6, 1, 64, _lens(13, 500, 5, 16), None, 1200, 3),
     ("float16", 4, 1, 512, _lens(14, 2, 100, 301), None, 777, 2),         # the key range in shares
     ("bfloat16", 8, 2, 512, _lens(15, 2, 64, 70), _lens(16, 2, 500, 900), 1030, 2),
-    ("float16", 3, 1, 512, _lens(17, 30, 1, 21), None, 450, 2),
-    ("bfloat16", 4, 1, 512, _lens(18, 30, 12, 24), None, 250, 2),
+    ("float16", 3, 1, 512, _lens(17, 30, 1, 21), None, 1001, 2),
+    ("bfloat16", 4, 1, 512, _lens(18, 30, 12, 24), None, 600, 2),
     ("bfloat16", 3, 1, 512, _lens(25, 90, 25, 31), None, 1001, 3),
     ("float16", 4, 1, 512, _lens(26, 3, 900, 1201), None, 555, 4),
 ]
@@ -51,8 +52,8 @@ def test_prefix(gpu, case, causal):
 
 
 @pytest.mark.parametrize("dtype,H,KV,D,B,P,pre,own", [
-    ("bfloat16", 4, 2, 256, 300, 6000, 2, 0), ("float16", 4, 1, 128, 300, 9001, 0, 0), ("float16", 4, 1, 128, 300, 60001, 4, 0),
-    ("float16", 8, 1, 64, 300, 16001, 4, 0), ("bfloat16", 4, 2, 512, 130, 3000, 2, 2)])
+    ("bfloat16", 4, 2, 256, 300, 6000, 0, 0), ("bfloat16", 4, 2, 256, 300, 20000, 4, 0), ("float16", 4, 1, 128, 300, 9001, 4, 0), ("float16", 4, 1, 128, 300, 60001, 4, 0),
+    ("float16", 8, 1, 64, 300, 16001, 4, 0), ("bfloat16", 4, 2, 512, 130, 3000, 2, 0)])
 def test_tokens_of_many_streams(gpu, dtype, H, KV, D, B, P, pre, own):
     """The prefix by the rows of all streams, their own keys by stream, each in the kernel its rule names, joined."""
     c = make(gpu, 32, dtype, H, KV, D, [1] * B, _lens(19, B, 0, 200), P)
@@ -63,7 +64,7 @@ def test_tokens_of_many_streams(gpu, dtype, H, KV, D, B, P, pre, own):
 
 BLOCKS = [
     # dtype, H, KV, D, q lengths, k lengths (None: the q's), q_block, n_sel, nw
-    ("float16", 3, 1, 256, [4500], None, 32, 10, 3),
+    ("float16", 3, 1, 256, [4500], None, 32, 12, 3),
     ("bfloat16", 4, 2, 256, _lens(20, 4, 60, 2900), None, 16, 14, 2),
     ("float16", 4, 1, 256, [3333], None, 64, 7, 0),
     ("float16", 4, 1, 256, [5555], None, 64, 11, 4),                      # 256 rows: two tiles of 128
@@ -74,7 +75,7 @@ BLOCKS = [
     ("bfloat16", 4, 1, 512, [1111], None, 33, 12, 2),
     ("float16", 4, 1, 512, [3000, 2000, 7], None, 33, 20, 4),             # 132 rows: a tile of 128, one of 4
     ("bfloat16", 4, 1, 512, [3000, 2000, 7], None, 24, 20, 3),
-    ("float16", 4, 1, 512, [640], [2000], 4, 6, 2),                       # 16 rows a list
+    ("float16", 4, 1, 512, [640], [2000], 4, 6, 0),                       # 16 rows a list
 ]
 
 
@@ -101,7 +102,7 @@ def test_blocks(gpu, case, causal):
 
 def test_quantized_pair(gpu):
     """Within half a step of each 128-dim scale of the context, rows outside the sequences zero; plain and in shares."""
-    for dtype, H, KV, D, ql, P in (("float16", 4, 1, 256, _lens(1, 3, 300, 701), 333), ("bfloat16", 4, 2, 128, [900, 3000], 400),
+    for dtype, H, KV, D, ql, P in (("float16", 4, 1, 256, _lens(1, 3, 300, 701), 1333), ("bfloat16", 4, 2, 128, [900, 3000], 400),
                                    ("float16", 4, 1, 512, [301, 100], 777)):
         c = make(gpu, 34, dtype, H, KV, D, ql, None, P)
         assert route_prefix(c)[3] >= 2
@@ -117,7 +118,8 @@ def test_quantized_pair(gpu):
 def test_replayed_with_other_lengths(gpu):
     import torch
     ql = _lens(1, 3, 300, 701)
-    c = make(gpu, 35, "float16", 4, 1, 256, ql, None, 333)
+    c = make(gpu, 35, "float16", 4, 1, 256, ql, None, 1333)
+    assert route_prefix(c)[3] == 4
     _run(c, 0.0625)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
@@ -171,7 +173,7 @@ def test_context_and_pair_at_once(gpu):
     import ctypes as C
     import e2mi
     import torch
-    for D, ql, P, nw in ((256, _lens(1, 3, 300, 701), 333, 4), (512, [301, 100], 777, 2), (128, [40, 3], 30, 0)):
+    for D, ql, P, nw in ((256, _lens(1, 3, 300, 701), 1333, 4), (512, [301, 100], 777, 2), (128, [40, 3], 30, 0)):
         c = make(gpu, 38, "float16", 4, 1, D, ql, None, P)
         plan = route_prefix(c)
         assert plan[3] == nw
