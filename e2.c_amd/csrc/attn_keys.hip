@@ -955,11 +955,13 @@ struct KeysPlan {
 // is begun is paid for: 150 groups are faster in 3 shares (450 workgroups, two rounds of a third each) than in 2 (300, two
 // rounds of a half). us a call, by the smallest number that fills the device | by this rule: one text of 1500 tokens of 4 heads
 // behind 4096 keys, head_dim 512 145 | 103, 256 73 | 59; 40 tokens of 8 heads on 4 over 8192 keys, 256 320 | 243, 128 142 | 125. Over 72 shapes it takes 1 % more than the best number of shares, the other 13 %.
-static int key_shares(double groups, int64_t tiles, int slots, double tile_us, double ctx_us, bool joined, int least, int most) {
+// step: beyond 8, multiples of it only.
+static int key_shares(double groups, int64_t tiles, int slots, double tile_us, double ctx_us, bool joined, int least, int most,
+                      int step = 1) {
     const int64_t end = std::min<int64_t>(most, tiles / least);
     int64_t best = 1;
     double best_us = 0.;
-    for (int64_t n = 1; n <= end; n++) {
+    for (int64_t n = 1; n <= end; n += n >= 8 ? step : 1) {
         const double us = ceil(groups * (double)n / slots - 1e-9) * (double)((tiles + n - 1) / n + 2) * tile_us +
                           (n > 1 || joined ? (double)n * ctx_us : 0.) + (n > 1 && !joined ? 7. : 0.);
         if (n == 1 || us < best_us) best = n, best_us = us;
@@ -985,7 +987,7 @@ static double few_bytes(int64_t rows, int64_t count, int64_t tiles, int D) { ret
 //   head_dim 512: 136 MB (64 tokens behind 4096) 27.5 | 30.2, 273 MB (128 tokens) 35.5 | 33.2; 8192 tokens, 16 blocks of keys
 //                 for each 16 rows 342 | 433, for each 24 347 | 222
 static double few_most(int D) { return D == 128 ? 350e6 : D == 256 ? 600e6 : 200e6; }
-static RowsPlan plan_rows(int64_t rows, int64_t count, double live, double all, int64_t tiles, int D, double values, int most, bool wide, bool joined) {
+static RowsPlan plan_rows(int64_t rows, int64_t count, double live, double all, int64_t tiles, int D, double values, int most, bool wide, bool joined, bool prefix) {
     RowsPlan p;
     p.nw = rows <= 64 ? 2 : rows <= 96 ? 3 : 4;
     // two row groups where four would not give every CU a workgroup even in shares (head_dim 512, 128 tokens behind 4096 keys:
@@ -1001,7 +1003,9 @@ static RowsPlan plan_rows(int64_t rows, int64_t count, double live, double all, 
         const int each = D == 512 ? 1 : p.nw == 2 && D <= 128 ? 4 : 2;
         p.parts = key_shares(groups, tiles, each * num_cus(), (double)R * each * D * 128 / 3.2e6, ctx_us, joined, 8, most);
     } else {
-        p.parts = key_shares(groups, tiles, num_cus(), D * 128 / 40e3, ctx_us, joined, 4, most);  // 40 GB/s a CU
+        // Workgroup i runs on XCD i % 8: in multiples of 8 shares, all that read one share of a prefix run on one XCD and its L2
+        // (8 tokens of 4 heads behind 16384 keys of 256, us a call: 32 shares 17.8, 31 29.2)
+        p.parts = key_shares(groups, tiles, num_cus(), D * 128 / 40e3, ctx_us, joined, 4, most, prefix ? 8 : 1);  // 40 GB/s a CU
     }
     // up to six tiles a wave, one workgroup's walk is shorter than a second launch to join shares (one token of 3 heads over
     // 531 keys of 256, us a call: 12.9 | 16.1 in four shares), unless there is one anyway (`joined`)
@@ -1023,9 +1027,9 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
     // 19.2 | 21.3, 4096 25.4 | 23.7, 16384 62.6 | 33.3; of 8 tokens 2048 27.1 | 36.8, 8192 62.7 | 55.2.
     p.apart = B > 1 && P > 0 && rows <= 64 && few_bytes(rows, (int64_t)B * KV, pre_tiles, D) > 200e6 + 1400.0 * Mq * H * D;
     const double all = (double)Mq * H, values = all * D;
-    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, KV, all, pre_tiles, D, values, kMaxKeyParts / 2, wide_takes(pre), true);
+    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, KV, all, pre_tiles, D, values, kMaxKeyParts / 2, wide_takes(pre), true, true);
     p.rows = plan_rows(rows, (int64_t)B * KV, (double)B * KV, all, own_tiles + (p.apart ? 0 : pre_tiles), D, values, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts,
-                       wide_takes(own) && (p.apart || wide_takes(pre)), p.apart);
+                       wide_takes(own) && (p.apart || wide_takes(pre)), p.apart, P > 0 && !p.apart);
     if (needs_copy(pre)) p.pad_pre = pad_bytes(P, KV, D);
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
@@ -1036,7 +1040,7 @@ static KeysPlan plan_blocks(int Mq, const KeySet &own, int B, int max_q, int H, 
     const int64_t NQ = ((int64_t)max_q + q_block - 1) / q_block;
     const double live = KV * std::min((double)NQ * B, std::max((double)B, (double)Mq / q_block + 0.5 * B));
     p.rows = plan_rows((int64_t)q_block * (H / KV), NQ * KV * B, live, INFINITY, 2 * (int64_t)n_sel, D, (double)Mq * H * D, kMaxKeyParts,
-                       wide_takes(own), false);
+                       wide_takes(own), false, false);
     p.rows.tiles *= NQ;
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
