@@ -1007,9 +1007,10 @@ static RowsPlan plan_rows(int64_t rows, int64_t count, double live, double all, 
         // (8 tokens of 4 heads behind 16384 keys of 256, us a call: 32 shares 17.8, 31 29.2)
         p.parts = key_shares(groups, tiles, num_cus(), D * 128 / 40e3, ctx_us, joined, 4, most, prefix ? 8 : 1);  // 40 GB/s a CU
     }
-    // up to six tiles a wave, one workgroup's walk is shorter than a second launch to join shares (one token of 3 heads over
-    // 531 keys of 256, us a call: 12.9 | 16.1 in four shares), unless there is one anyway (`joined`)
-    if (!p.nw && tiles <= 24 && !joined) p.parts = 1;
+    // a short walk (up to six tiles a wave; at head_dim 512, of half the waves and twice the tile, three) takes less than a
+    // second launch to join shares, unless there is one anyway (`joined`): one token of 3 heads over 531 keys, one | four shares,
+    // head_dim 256 14.6 | 17.6, 512 29.2 | 18.9 (300 keys: 21.5 | 19.1)
+    if (!p.nw && tiles <= (D == 512 ? 6 : 24) && !joined) p.parts = 1;
     return p;
 }
 

@@ -25,6 +25,7 @@ def test_shares_fill_rounds():
     assert prefix(1500, 1500, 4096, 1, 1500, 1500, 4, 1, 512)[3:5] == [4, 5]     # 47 row tiles: 235 workgroups, one a CU
     assert prefix(40, 40 * 8192, 8, 40, 1, 8192, 8, 4, 256)[3:5] == [0, 3]       # 160: 480, two rounds
     assert prefix(1, 0, 531, 1, 1, 0, 3, 1, 256)[3:5] == [0, 1]                  # a short walk in one launch
+    assert prefix(1, 0, 531, 1, 1, 0, 3, 1, 512)[4] > 1
     assert prefix(1, 0, 8192, 1, 1, 0, 4, 1, 256)[4] >= 32
     assert prefix(8, 8 * 64, 16384, 8, 1, 64, 4, 1, 256)[3:5] == [0, 32]         # of a shared prefix in multiples of 8
     for D in (64, 128, 256, 512):
