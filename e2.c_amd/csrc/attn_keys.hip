@@ -941,6 +941,7 @@ __global__ __launch_bounds__(256) void k_keys_merge(KeysArgs a) {
 struct RowsPlan {
     int nw = 0, parts = 1;
     int64_t tiles = 0;  // per sequence and kv head
+    double us = 0.;     // what the launch takes, about (and the join that it asks for)
 };
 struct KeysPlan {
     bool apart = false;  // the prefix by rows of all sequences, their own keys by sequence
@@ -956,17 +957,14 @@ struct KeysPlan {
 // rounds of a half). us a call, by the smallest number that fills the device | by this rule: one text of 1500 tokens of 4 heads
 // behind 4096 keys, head_dim 512 145 | 103, 256 73 | 59; 40 tokens of 8 heads on 4 over 8192 keys, 256 320 | 243, 128 142 | 125. Over 72 shapes it takes 1 % more than the best number of shares, the other 13 %.
 // step: beyond 8, multiples of it only.
-static int key_shares(double groups, int64_t tiles, int slots, double tile_us, double ctx_us, bool joined, int least, int most,
-                      int step = 1) {
+static void key_shares(RowsPlan &p, double groups, int64_t tiles, int slots, double tile_us, double ctx_us, bool joined, int least,
+                       int most, int step = 1) {
     const int64_t end = std::min<int64_t>(most, tiles / least);
-    int64_t best = 1;
-    double best_us = 0.;
-    for (int64_t n = 1; n <= end; n += n >= 8 ? step : 1) {
+    for (int64_t n = 1; n == 1 || n <= end; n += n >= 8 ? step : 1) {
         const double us = ceil(groups * (double)n / slots - 1e-9) * (double)((tiles + n - 1) / n + 2) * tile_us +
                           (n > 1 || joined ? (double)n * ctx_us : 0.) + (n > 1 && !joined ? 7. : 0.);
-        if (n == 1 || us < best_us) best = n, best_us = us;
+        if (n == 1 || us < p.us) p.parts = (int)n, p.us = us;
     }
-    return (int)best;
 }
 
 // k_keys_wide's offsets into V^T within a wave's rows (up to 128) are 32 bits: caches past 8 M columns take k_keys_few
@@ -999,18 +997,19 @@ static RowsPlan plan_rows(int64_t rows, int64_t count, double live, double all, 
     const double groups = std::min((double)p.tiles * live, std::max(live, all / R + 0.5 * live));
     const double ctx_us = values * 8. / 4e6;  // 4 TB/s
     if (p.nw) {
-        // workgroups a CU: one at head_dim 512 (LDS), four of two groups at 128 and below; 3.2 TFLOP/s a CU
+        // workgroups a CU: one at head_dim 512 (LDS), four of two groups at 128 and below. 3.2 TFLOP/s a CU; 2.5 of
+        // smaller tiles, whose waves are fewer
         const int each = D == 512 ? 1 : p.nw == 2 && D <= 128 ? 4 : 2;
-        p.parts = key_shares(groups, tiles, each * num_cus(), (double)R * each * D * 128 / 3.2e6, ctx_us, joined, 8, most);
+        key_shares(p, groups, tiles, each * num_cus(), (double)R * each * D * 128 / (p.nw == 4 ? 3.2e6 : 2.5e6), ctx_us, joined, 8, most);
     } else {
+        // A short walk (up to six tiles a wave; at head_dim 512, of half the waves and twice the tile, three) takes less than a
+        // second launch to join shares, unless there is one anyway (`joined`): one token of 3 heads over 531 keys, one | four
+        // shares, head_dim 256 14.6 | 17.6, 512 29.2 | 18.9 (300 keys: 21.5 | 19.1).
         // Workgroup i runs on XCD i % 8: in multiples of 8 shares, all that read one share of a prefix run on one XCD and its L2
-        // (8 tokens of 4 heads behind 16384 keys of 256, us a call: 32 shares 17.8, 31 29.2)
-        p.parts = key_shares(groups, tiles, num_cus(), D * 128 / 40e3, ctx_us, joined, 4, most, prefix ? 8 : 1);  // 40 GB/s a CU
+        // (8 tokens of 4 heads behind 16384 keys of 256, us a call: 32 shares 17.8, 31 29.2). 40 GB/s a CU.
+        const bool brief = tiles <= (D == 512 ? 6 : 24) && !joined;
+        key_shares(p, groups, tiles, num_cus(), D * 128 / 40e3, ctx_us, joined, 4, brief ? 1 : most, prefix ? 8 : 1);
     }
-    // a short walk (up to six tiles a wave; at head_dim 512, of half the waves and twice the tile, three) takes less than a
-    // second launch to join shares, unless there is one anyway (`joined`): one token of 3 heads over 531 keys, one | four shares,
-    // head_dim 256 14.6 | 17.6, 512 29.2 | 18.9 (300 keys: 21.5 | 19.1)
-    if (!p.nw && tiles <= (D == 512 ? 6 : 24) && !joined) p.parts = 1;
     return p;
 }
 
@@ -1023,14 +1022,19 @@ static KeysPlan plan_prefix(int Mq, const KeySet &own, const KeySet &pre, int B,
     const int G = H / KV, P = pre.rows;
     const int64_t own_tiles = own.rows ? ((int64_t)max_k + 31) / 32 : 0, pre_tiles = ((int64_t)P + 31) / 32;
     const int64_t rows = (int64_t)max_q * G;
-    // Sequences of few rows share the prefix's tiles where reading it for each costs more than the join of the shares, which
-    // follows the rows' contexts. us a call, each | shared: head_dim 256, 64 sequences of 1 token of 4 heads behind 2048 keys
-    // 19.2 | 21.3, 4096 25.4 | 23.7, 16384 62.6 | 33.3; of 8 tokens 2048 27.1 | 36.8, 8192 62.7 | 55.2.
-    p.apart = B > 1 && P > 0 && rows <= 64 && few_bytes(rows, (int64_t)B * KV, pre_tiles, D) > 200e6 + 1400.0 * Mq * H * D;
-    const double all = (double)Mq * H, values = all * D;
-    if (p.apart) p.pre = plan_rows((int64_t)Mq * G, KV, KV, all, pre_tiles, D, values, kMaxKeyParts / 2, wide_takes(pre), true, true);
-    p.rows = plan_rows(rows, (int64_t)B * KV, (double)B * KV, all, own_tiles + (p.apart ? 0 : pre_tiles), D, values, p.apart ? kMaxKeyParts / 2 : kMaxKeyParts,
-                       wide_takes(own) && (p.apart || wide_takes(pre)), p.apart, P > 0 && !p.apart);
+    const double all = (double)Mq * H, values = all * D, count = (double)B * KV;
+    p.rows = plan_rows(rows, (int64_t)B * KV, count, all, own_tiles + pre_tiles, D, values, kMaxKeyParts, wide_takes(own) && wide_takes(pre),
+                       false, P > 0);
+    // Sequences of few rows share the prefix's tiles where reading it for each takes longer than two launches, the prefix by all
+    // rows together and the own keys, and the join of their shares (16 us of starts among them). us a call, each | shared: head_dim
+    // 256, 64 sequences of 1 token of 4 heads behind 2048 keys 17.2 | 19.9, 16384 58 | 30; of 16 tokens 4096 47.3 | 53.9, head_dim
+    // 512, 200 of 2 tokens of 8 heads on 2 behind 1024 92.0 | 55.7. Over 180 shapes 0.4 % more than the better of the two.
+    if (B > 1 && P > 0 && rows <= 64) {
+        const RowsPlan pre_rows = plan_rows((int64_t)Mq * G, KV, KV, all, pre_tiles, D, values, kMaxKeyParts / 2, wide_takes(pre), true, true);
+        const RowsPlan own_rows = plan_rows(rows, (int64_t)B * KV, count, all, own_tiles, D, values, kMaxKeyParts / 2, wide_takes(own), true,
+                                            false);
+        if (pre_rows.us + own_rows.us + 16. < p.rows.us) p.apart = true, p.pre = pre_rows, p.rows = own_rows;
+    }
     if (needs_copy(pre)) p.pad_pre = pad_bytes(P, KV, D);
     if (needs_copy(own)) p.pad_own = pad_bytes(own.rows, KV, D);
     return p;
