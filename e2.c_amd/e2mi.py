@@ -771,7 +771,7 @@ def _torch():
 
 def _kind(name, t):
     """The library's code of a tensor's type, and its device, which has to be the current one."""
-    codes, _, device, _, _, _ = _torch()
+    codes, _, device = _torch()[:3]
     kind, dev = codes.get(t.dtype), t.get_device()
     if kind is None:
         raise E2MIError(f"{name}: needs f16, bf16 or f32 rows, got {t.dtype}")
@@ -841,13 +841,14 @@ def rope(q, k, pos, freqs, H, KV, layout="half", magnitude=1.0, inverse=False, q
     D = _head_dim("rope", x, heads, heads)
     kind, dev = _kind("rope", x)
     dtype, (M, width) = x.dtype, x.shape
+    like = torch.empty_like
     pq = pk = po = pt = None
     lq = lk = lo = lt = nq = nk = 0
     if q is not None:
         pq, lq = _rows("rope", q, M, width, dtype, dev)
         nq = H
         if q_out is None:
-            q_out = _new(stream, q.new_empty, (M, width))
+            q_out = like(q) if stream is None else _new(stream, like, q)
             po, lo = q_out.data_ptr(), width
         else:
             po, lo = _rows("rope", q_out, M, width, dtype, dev)
@@ -855,7 +856,7 @@ def rope(q, k, pos, freqs, H, KV, layout="half", magnitude=1.0, inverse=False, q
         pk, lk = _rows("rope", k, M, KV * D, dtype, dev)
         nk = KV
         if k_out is None:
-            k_out = _new(stream, k.new_empty, (M, KV * D))
+            k_out = like(k) if stream is None else _new(stream, like, k)
             pt, lt = k_out.data_ptr(), KV * D
         else:
             pt, lt = _rows("rope", k_out, M, KV * D, dtype, dev)
@@ -907,7 +908,7 @@ def _workspace(name, need, workspace, like, stream, dev):
     if workspace is None:
         if not need:
             return None, None, 0
-        _, _, _, _, uint8, empty = _torch()
+        uint8, empty = _torch()[4:6]
         workspace = empty(need, dtype=uint8, device=like.device) if stream is None else _new(stream, empty, need, dtype=uint8, device=like.device)
         return workspace, workspace.data_ptr(), need
     if workspace.get_device() != dev or not workspace.is_contiguous():
